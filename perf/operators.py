@@ -9,9 +9,9 @@ them, beside their plain forms in elementary tensor operations.
                pages taken from a list of free ones;
 ``verify``     drafted tokens against the target's probabilities: how many stay, and the token behind them.
 
-The cache: a page of one key/value head is one tile of bytes: ``page_size`` rows of ``head_dim / 2`` bytes
-(channel 2i in the low half of byte i), then for every row and group of 32 channels (the last may be
-shorter) two bfloat16 numbers (step, middle).  A code c stands for middle + step * (c - 8).
+The cache: a page of one key/value head is one tile of bytes: for every group of 32 channels (the last may
+be shorter) the codes of ``page_size`` rows (two channels a byte, channel 2i in the low half of byte i), then
+for every row its groups' two bfloat16 numbers (step, middle).  A code c stands for middle + step * (c - 8).
 """
 import math
 
@@ -202,16 +202,29 @@ def _values(code, params):
 def _pack(code, params):
     """Tiles of bytes [pages, heads, tile] of codes [pages, heads, page, head_dim] and their parameters."""
     code = code.to(torch.uint8)
-    rows = (code[..., 0::2] | (code[..., 1::2] << 4)).flatten(-2)
-    return torch.cat([rows, params.contiguous().view(torch.uint8).flatten(2)], -1).contiguous()
+    rows = code[..., 0::2] | (code[..., 1::2] << 4)
+    whole = code.shape[-1] // GROUP * (GROUP // 2)               # bytes of a row's whole groups
+    parts = [rows[..., :whole].unflatten(-1, (-1, GROUP // 2)).transpose(-2, -3).flatten(2),
+             rows[..., whole:].flatten(2), params.contiguous().view(torch.uint8).flatten(2)]
+    return torch.cat(parts, -1).contiguous()
+
+
+def _tile_parts(tiles, page, head_dim):
+    """Views of tiles [..., tile]: codes of the whole groups [..., groups, page, 16], of the short one [..., page,
+    bytes] and the parameters' bytes [..., page, 4 * groups]."""
+    whole = head_dim // GROUP * page * (GROUP // 2)
+    codes = page * head_dim // 2
+    return (tiles[..., :whole].unflatten(-1, (head_dim // GROUP, page, GROUP // 2)),
+            tiles[..., whole:codes].unflatten(-1, (page, head_dim % GROUP // 2)),
+            tiles[..., codes:].unflatten(-1, (page, -1)))
 
 
 def _unpack(tiles, page, head_dim):
     """Codes and parameters of tiles [..., tile]."""
-    rows = tiles[..., :page * head_dim // 2].unflatten(-1, (page, head_dim // 2))
+    whole, short, params = _tile_parts(tiles, page, head_dim)
+    rows = torch.cat([whole.transpose(-2, -3).flatten(-2), short], -1)
     code = torch.stack([rows & 15, rows >> 4], -1).flatten(-2)
-    params = tiles[..., page * head_dim // 2:].contiguous().view(torch.bfloat16)
-    return code, params.unflatten(-1, (page, -1, 2))
+    return code, params.contiguous().view(torch.bfloat16).unflatten(-1, (-1, 2))
 
 
 def _plain_append(s):
@@ -224,9 +237,12 @@ def _plain_append(s):
         code, params = _quantize(x[rows].unflatten(1, (h, d)))
         c = code.to(torch.uint8)
         at = (slots // page, slots % page)
-        tiles[..., :page * d // 2].unflatten(-1, (page, d // 2))[at[0], :, at[1]] = c[..., 0::2] | (c[..., 1::2] << 4)
-        tiles[..., page * d // 2:].unflatten(-1, (page, -1))[at[0], :, at[1]] = \
-            params.contiguous().view(torch.uint8).flatten(2)
+        byte = c[..., 0::2] | (c[..., 1::2] << 4)
+        whole, short, pairs = _tile_parts(tiles, page, d)
+        cut = d // GROUP * (GROUP // 2)
+        whole[at[0], :, :, at[1]] = byte[..., :cut].unflatten(-1, (-1, GROUP // 2))
+        short[at[0], :, at[1]] = byte[..., cut:]
+        pairs[at[0], :, at[1]] = params.contiguous().view(torch.uint8).flatten(2)
         back[rows] = _values(code, params).flatten(1)
         out.append(back)
     return out
@@ -378,7 +394,9 @@ def exact(case, seed):
         cached = []
         for tiles in (s["k_tiles"][pages], s["v_tiles"][pages]):
             raw = tiles.permute(1, 0, 2)                                        # [kv, pages, tile]
-            byte = raw[..., :page * d // 2].reshape(kv, -1, d // 2)[:, :total]
+            edge = [page * min(g * GROUP, d) // 2 for g in range(-(-d // GROUP) + 1)]
+            byte = torch.cat([raw[..., i:j].reshape(kv, raw.shape[1] * page, -1) for i, j in zip(edge, edge[1:])], -1)
+            byte = byte[:, :total]
             par = raw[..., page * d // 2:].contiguous().view(torch.bfloat16).reshape(kv, -1, -(-d // GROUP), 2)
             par = par[:, :total].double()
             value = torch.empty(kv, total, d, dtype=torch.float64, device=raw.device)
