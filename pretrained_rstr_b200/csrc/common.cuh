@@ -32,6 +32,7 @@
 #define PRB_S_PAGE_RANGE 4       // block-table entry outside the pool or missing
 #define PRB_S_WAIT_TIMEOUT 5     // a bounded wait on a barrier gave up
 #define PRB_S_ROW_RANGE 6        // a row index outside its tensor
+#define PRB_S_LOGITS 7           // a row of logits without a finite largest one, or with NaN
 
 __device__ __forceinline__ void prb_set_status(int* status, int code, int a, int b, int c) {
     if (status == nullptr) return;

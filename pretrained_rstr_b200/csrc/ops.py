@@ -9,6 +9,7 @@ non-zero return code into an exception that names the refused argument.
 from __future__ import annotations
 
 import ctypes
+import math
 from ctypes import c_float, c_int, c_long, c_void_p
 from typing import Optional
 
@@ -33,6 +34,7 @@ STATUS_TEXT = {
     4: "block-table entry missing or outside the pool (token index, position, page)",
     5: "a bounded wait inside a kernel gave up (kernel id, block, stage)",
     6: "row index outside its tensor (row, index, rows)",
+    7: "a row of logits without a finite largest one, or with NaN (row, request)",
 }
 
 
@@ -241,6 +243,14 @@ def _declare(h: ctypes.CDLL) -> None:
     h.prb_mmem_scan_supports.argtypes = [I]
     h.prb_mmem_scan.argtypes = [P, L, P, P, P, L, I, I, I, I, I, I, P, P, P, P, P, P, P, P, P, P,
                                 I, I, I, I, I, I, F, F, F, F, I, P, P, P, P, P, I, I, P]
+    h.prb_kv_append_4bit.argtypes = [P, P, P, L, P, L, P, I, I, I, I, I, I, P, P]
+    h.prb_kv_read_4bit.argtypes = [P, L, P, L, P, P, P, I, I, I, I, I, I, P, P]
+    h.prb_attention_4bit.argtypes = [P, L, P, L] + [P] * 8 + [I] * 10 + [F, I, I, I, I, P, P]
+    h.prb_step_tables.argtypes = [P] * 13 + [I] * 6 + [P, P]
+    h.prb_verify_drafts.argtypes = [P, P, P, L, P, P, P, L, P, P, I, I, I, P, P]
+    for name in ("prb_kv_append_4bit", "prb_kv_read_4bit", "prb_attention_4bit", "prb_step_tables",
+                 "prb_verify_drafts"):
+        getattr(h, name).restype = c_int
     for name in ("prb_lru_max_taps", "prb_lru_conv", "prb_lru_gates", "prb_lru_scan",
                  "prb_mmem_supports", "prb_mmem_step", "prb_mmem_segment",
                  "prb_mmem_max_segments", "prb_mmem_scan_supports", "prb_mmem_scan"):
@@ -2664,3 +2674,258 @@ class StateSpace:
         if arrived.numel() < self.n_requests:
             raise KernelArgumentError("ssm_step: one counter per request")
         _check(lib().prb_ssm_step(*self._args, _p(arrived), self.out_dtype, _stream()), "ssm_step")
+
+
+# ------------------------------------------- a paged cache held in 4 bits, steps with drafted tokens
+# (These calls are most of what a small step costs, so their checks are a few attribute reads a tensor, and the stream
+# is asked for by its number.)
+CACHE4_MAX_HEAD_DIM, CACHE4_MAX_PAGE = 128, 1024
+ATTENTION_4BIT_MAX_PARTS = 8
+STEP_TABLES_MAX_REQUESTS = 4096         # most requests of a step that step_tables takes
+VERIFY_DRAFTS_MAX_TOKENS = 31           # most drafted tokens of a request that verify_drafts takes
+
+
+def _one_device(what: str, names, tensors) -> int:
+    """The CUDA device that all of ``tensors`` (None is skipped) lie on."""
+    device = None
+    for i, t in enumerate(tensors):
+        if t is None:
+            continue
+        d = t.get_device()
+        if d != device:
+            if d < 0:
+                raise KernelArgumentError(f"{what}: {names.split()[i]} is not on a CUDA device")
+            if device is not None:
+                raise KernelArgumentError(f"{what}: {names.split()[i]} is on device {d}, the others on device {device}")
+            device = d
+    return device
+
+
+def _launch_on(device: int, what: str, name: str, *args) -> None:
+    """The library's ``name(*args, stream)`` on ``device``'s current stream, whatever the current device is."""
+    call = getattr(lib(), name)
+    if device == torch._C._cuda_getDevice():
+        code = call(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            code = call(*args, torch._C._cuda_getCurrentRawStream(device))
+    _check(code, what)
+
+
+def _ints(what: str, name: str, t, n: int) -> int:
+    """The address of a contiguous int32 tensor of at least ``n`` numbers."""
+    if t.dtype is not torch.int32 or t.numel() < n or not t.is_contiguous():
+        raise KernelArgumentError(f"{what}: {name} must be contiguous int32 with at least {n} numbers, is "
+                                  f"{t.dtype} {list(t.shape)}")
+    return t.data_ptr()
+
+
+def _status4(what: str, status):
+    return None if status is None else _ints(what, "status", status, 4)
+
+
+def _matrix4(what: str, name: str, t, rows: int, width: int) -> int:
+    """The element type's code of [>= rows, width] with neighbouring columns."""
+    if t.dim() != 2 or t.shape[1] != width or t.shape[0] < rows or (width > 1 and t.stride(1) != 1) or t.stride(0) < 0:
+        raise KernelArgumentError(f"{what}: {name} must be [tokens, {width}] with neighbouring columns and at least "
+                                  f"{rows} rows, is {list(t.shape)}")
+    return dtype_code(t.dtype)
+
+
+def cache4_tile_bytes(head_dim: int, page_size: int) -> int:
+    """Bytes of a page of one key/value head in a cache held in 4 bits.  Head sizes are multiples of 16 up to 128,
+    pages multiples of 16 positions up to 1,024."""
+    if head_dim % 16 or not 16 <= head_dim <= CACHE4_MAX_HEAD_DIM or page_size % 16 or \
+            not 16 <= page_size <= CACHE4_MAX_PAGE:
+        raise KernelArgumentError(f"a cache held in 4 bits takes head sizes that are multiples of 16 up to "
+                                  f"{CACHE4_MAX_HEAD_DIM} and pages of a multiple of 16 positions up to "
+                                  f"{CACHE4_MAX_PAGE}; asked for {head_dim} and {page_size}")
+    return page_size * (head_dim // 2 + 4 * ((head_dim + 31) // 32))
+
+
+def _tiles4(what: str, k_tiles, v_tiles, head_dim: int, page_size: int):
+    tile = cache4_tile_bytes(head_dim, page_size)
+    for name, t in (("k_tiles", k_tiles), ("v_tiles", v_tiles)):
+        if t.dtype is not torch.uint8 or t.dim() != 3 or t.shape[2] != tile or not t.is_contiguous():
+            raise KernelArgumentError(f"{what}: {name} must be contiguous uint8 [pages, heads, {tile}], is {t.dtype} "
+                                      f"{list(t.shape)}")
+    pages, heads, _tile = k_tiles.shape
+    if v_tiles.shape[0] != pages or v_tiles.shape[1] != heads:
+        raise KernelArgumentError(f"{what}: k_tiles and v_tiles differ in shape")
+    return pages, heads
+
+
+def _rows_4bit(what: str, call, first: bool, names, a, b, k_tiles, v_tiles, slots, n_tokens, head_dim, page_size, status):
+    device = _one_device(what, names + " k_tiles v_tiles slots status", (a, b, k_tiles, v_tiles, slots, status))
+    pages, heads = _tiles4(what, k_tiles, v_tiles, head_dim, page_size)
+    if n_tokens < 0:
+        raise KernelArgumentError(f"{what}: n_tokens is below zero")
+    a_name, b_name = names.split()
+    code = _matrix4(what, a_name, a, n_tokens, heads * head_dim)
+    if _matrix4(what, b_name, b, n_tokens, heads * head_dim) != code:
+        raise KernelArgumentError(f"{what}: {a_name} and {b_name} differ in type")
+    rows = (a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0))
+    tiles = (k_tiles.data_ptr(), v_tiles.data_ptr())
+    slots, status = _ints(what, "slots", slots, n_tokens), _status4(what, status)
+    _launch_on(device, what, call, *(tiles + rows if first else rows + tiles), slots, n_tokens, heads,
+               head_dim, page_size, pages, code, status)
+
+
+def kv_append_4bit(k_tiles, v_tiles, k, v, slots, n_tokens: int, head_dim: int, page_size: int, status) -> None:
+    """Round the step's keys and values to 4 bits at their cache slots.  ``k_tiles`` / ``v_tiles``: uint8 [pages,
+    kv_heads, ``cache4_tile_bytes(head_dim, page_size)``]; ``k`` / ``v``: [T, kv_heads * head_dim] bfloat16 or float32,
+    may be column slices of a wider tensor; ``slots`` int32: page * page_size + place of each token, below zero = none.
+    No two tokens have one slot.
+
+    Of every 32 channels (the last group may be shorter) the cache keeps step = (largest - smallest) / 15 and middle =
+    smallest + 8 step in bfloat16 and per channel the nearest of 16 codes; code c reads back as middle + step * (c - 8).
+    A group whose step would be below 2^-126 reads back as its smallest number; one that holds an infinity or a NaN
+    reads back as NaN."""
+    _rows_4bit("kv_append_4bit", "prb_kv_append_4bit", True, "k v", k, v, k_tiles, v_tiles, slots, n_tokens, head_dim,
+               page_size, status)
+
+
+def kv_read_4bit(k_out, v_out, k_tiles, v_tiles, slots, n_tokens: int, head_dim: int, page_size: int, status) -> None:
+    """What a cache held in 4 bits stands for at ``slots`` (see :func:`kv_append_4bit`): rows of ``k_out`` / ``v_out``
+    [T, kv_heads * head_dim], float32 (exact but for a last rounding to 32 bits) or bfloat16.  Rows whose slot is below
+    zero stay as they were."""
+    _rows_4bit("kv_read_4bit", "prb_kv_read_4bit", False, "k_out v_out", k_out, v_out, k_tiles, v_tiles, slots, n_tokens,
+               head_dim, page_size, status)
+
+
+def attention_4bit(out, q, k_tiles, v_tiles, block_table, positions, tile_req, tile_row0, tile_rows, tile_most: int,
+                   n_heads: int, head_dim: int, page_size: int, scale: float, window, max_context: int, status,
+                   tile_count=None, parts: int = 0) -> None:
+    """Causal attention of tiles of tokens over their requests' pages of a cache held in 4 bits
+    (:func:`kv_append_4bit`), the tokens' own keys and values included.
+
+    ``q``, ``out``: [T, n_heads * head_dim], both bfloat16 or both float32 (may be column slices); ``block_table``
+    int32 [requests, pages a request]; ``positions`` int32 [T].  Tile i: tokens ``tile_row0[i]`` to ``tile_row0[i] +
+    tile_rows[i] - 1``, neighbours of request ``tile_req[i]`` (a row of the block table) at neighbouring positions;
+    no tile has more than ``tile_most`` of them, and 128 rows (tokens times the heads that share a key/value head) a
+    tile are about what a portion of a prompt should be cut into; a decoded token is a tile of one.  ``tile_count``:
+    int32 on the device, how many of the tiles count (all by default).  ``window``: a token sees its last ``window``
+    positions only.  ``max_context``: the most positions a request holds (the keys are cut into parts by it).
+    ``parts``: CTAs that share a tile's keys (0: the kernel's rule).  Rows of no tile stay as they were."""
+    what = "attention_4bit"
+    device = _one_device(what, "out q k_tiles v_tiles block_table positions tile_req tile_row0 tile_rows tile_count status",
+                         (out, q, k_tiles, v_tiles, block_table, positions, tile_req, tile_row0, tile_rows, tile_count,
+                          status))
+    pages, kv_heads = _tiles4(what, k_tiles, v_tiles, head_dim, page_size)
+    if n_heads < 1 or n_heads % kv_heads:
+        raise KernelArgumentError(f"{what}: {n_heads} query heads are not a multiple of {kv_heads} key/value heads")
+    if window is not None and window < 1:
+        raise KernelArgumentError(f"{what}: a window holds at least the token itself")
+    if tile_most < 1 or max_context < 1 or not 0 <= parts <= ATTENTION_4BIT_MAX_PARTS or not math.isfinite(scale):
+        raise KernelArgumentError(f"{what}: tile_most and max_context are at least 1, parts 0 to "
+                                  f"{ATTENTION_4BIT_MAX_PARTS}, scale is finite; got {tile_most}, {max_context}, {parts}, "
+                                  f"{scale}")
+    width = n_heads * head_dim
+    tokens = q.shape[0]
+    code = _matrix4(what, "q", q, 0, width)
+    if _matrix4(what, "out", out, tokens, width) != code:
+        raise KernelArgumentError(f"{what}: q and out differ in type")
+    q_at, out_at = q.data_ptr(), out.data_ptr()
+    if q_at == out_at and tokens > 0:
+        raise KernelArgumentError(f"{what}: out must not be q")
+    if block_table.dim() != 2:
+        raise KernelArgumentError(f"{what}: block_table must be [requests, pages a request]")
+    requests, wide = block_table.shape
+    n_tiles = tile_req.numel()
+    _launch_on(device, what, "prb_attention_4bit",
+               out_at, out.stride(0), q_at, q.stride(0), k_tiles.data_ptr(), v_tiles.data_ptr(),
+               _ints(what, "block_table", block_table, 0), _ints(what, "positions", positions, tokens),
+               _ints(what, "tile_req", tile_req, 0), _ints(what, "tile_row0", tile_row0, n_tiles),
+               _ints(what, "tile_rows", tile_rows, n_tiles),
+               None if tile_count is None else _ints(what, "tile_count", tile_count, 1), n_tiles, tile_most, tokens,
+               requests, n_heads, kv_heads, head_dim, page_size, wide, pages, scale, window or 0, max_context, parts, code,
+               _status4(what, status))
+
+
+def step_tables(rows, held, brought, tables, page_size: int, q_start, kv_len, positions, seq_of_token, slots, block_table,
+                status, free_pages=None, free_start=None, free_next=None) -> None:
+    """The arrays of a step (as ``engine.batch`` lays them out) from the requests' lengths, on the device.
+
+    Request b (row ``rows[b]`` of ``tables`` int32 [rows, pages a request]; no two requests have one row) holds
+    ``held[b]`` tokens and brings ``brought[b]`` (none is fine).  Written: ``q_start`` [requests + 1], ``kv_len``
+    [requests]; per token row ``positions``, ``seq_of_token``, ``slots`` (rows behind the last token get 0, -1, -1);
+    ``block_table`` [requests, pages a request]: the request's pages up to its last new token, -1 behind them.  Pages a
+    request grows into come from ``free_pages`` [``free_start[0]`` ...], in the requests' order, and are put into
+    ``tables`` too; ``free_next[0]`` becomes the place behind the last one taken (not ``free_start`` itself: the caller
+    has the two take turns).  Without ``free_pages`` the rows of ``tables`` hold the pages already (the cache manager
+    reserves them on the host).
+
+    In the status word: a request whose row or lengths do not fit (it brings nothing, its block table row stays
+    empty), a page that is missing (the slot is -1), more tokens than token rows (those behind are left out)."""
+    what = "step_tables"
+    device = _one_device(what, "rows held brought tables q_start kv_len positions seq_of_token slots block_table status "
+                         "free_pages free_start free_next",
+                         (rows, held, brought, tables, q_start, kv_len, positions, seq_of_token, slots, block_table, status,
+                          free_pages, free_start, free_next))
+    n, cap = held.numel(), positions.numel()
+    if not 1 <= n <= STEP_TABLES_MAX_REQUESTS:
+        raise KernelArgumentError(f"{what}: takes 1 to {STEP_TABLES_MAX_REQUESTS} requests, got {n}")
+    if page_size < 1:
+        raise KernelArgumentError(f"{what}: page_size must be at least 1")
+    if tables.dim() != 2 or block_table.dim() != 2 or tables.shape[1] < 1:
+        raise KernelArgumentError(f"{what}: tables and block_table must be [rows, pages a request]")
+    lanes, wide = tables.shape
+    if block_table.shape[0] < n or block_table.shape[1] != wide:
+        raise KernelArgumentError(f"{what}: block_table must have {n} rows of {wide} pages, is {list(block_table.shape)}")
+    t_at, b_at = _ints(what, "tables", tables, 0), _ints(what, "block_table", block_table, 0)
+    if t_at < b_at + 4 * n * wide and b_at < t_at + 4 * lanes * wide:
+        raise KernelArgumentError(f"{what}: block_table and tables are two tensors")
+    free_at, start_at, next_at, n_free = None, None, None, 0
+    if free_pages is not None:
+        if free_start is None or free_next is None:
+            raise KernelArgumentError(f"{what}: free_pages come with free_start and free_next")
+        free_at, n_free = _ints(what, "free_pages", free_pages, 0), free_pages.numel()
+        start_at, next_at = _ints(what, "free_start", free_start, 1), _ints(what, "free_next", free_next, 1)
+        if start_at == next_at:
+            raise KernelArgumentError(f"{what}: free_next must not be free_start")
+    _launch_on(device, what, "prb_step_tables",
+               _ints(what, "rows", rows, n), _ints(what, "held", held, n), _ints(what, "brought", brought, n), t_at,
+               free_at, start_at, next_at, _ints(what, "q_start", q_start, n + 1), _ints(what, "kv_len", kv_len, n),
+               _ints(what, "positions", positions, 0), _ints(what, "seq_of_token", seq_of_token, cap),
+               _ints(what, "slots", slots, cap), b_at, n, lanes, cap, wide, page_size, n_free, _status4(what, status))
+
+
+def verify_drafts(tokens, accepted, logits, row_start, drafted, uniforms, temperature, status, draft_probs=None) -> None:
+    """Which drafted tokens stay, and the token behind them.
+
+    Request b has the rows ``row_start[b]`` to ``row_start[b + 1] - 1`` of ``logits`` float32 [rows, vocabulary]: one
+    more than it drafted tokens (at most ``VERIFY_DRAFTS_MAX_TOKENS``); row i of a request is the target's answer
+    behind its i-th drafted token, and ``drafted[row]`` the token that the draft put there (of a request's last row:
+    not read).  ``temperature`` float32 [requests]: the target's probabilities are softmax(logits / temperature); 0 or
+    less is greedy.  ``draft_probs`` float32 [rows, vocabulary]: what the draft drew each token from (None: the draft
+    was sure of its tokens).  ``uniforms`` float32 [rows, 2], in [0, 1): the first decides whether the row's token
+    stays (u * draft's probability < target's), the second draws the token where the row is the last to be read: from
+    what the target's probabilities exceed the draft's by where a token was refused, from the target's behind the last
+    drafted token, the lowest index at which the running sum passes the number's share of the whole.
+
+    Written: ``accepted[b]``: drafted tokens that stay; ``tokens`` int32 [rows]: they and the token behind them, -1 in
+    the request's rows beyond."""
+    what = "verify_drafts"
+    device = _one_device(what, "tokens accepted logits row_start drafted uniforms temperature status draft_probs",
+                         (tokens, accepted, logits, row_start, drafted, uniforms, temperature, status, draft_probs))
+    for name, t in (("logits", logits), ("draft_probs", draft_probs)):
+        if t is not None and (t.dtype is not torch.float32 or t.dim() != 2 or t.stride(0) < 0 or
+                              (t.shape[1] > 1 and t.stride(1) != 1)):
+            raise KernelArgumentError(f"{what}: {name} must be float32 [rows, vocabulary] with neighbouring columns")
+    rows, vocab = logits.shape
+    if draft_probs is not None and (draft_probs.shape[0] != rows or draft_probs.shape[1] != vocab):
+        raise KernelArgumentError(f"{what}: draft_probs and logits differ in shape")
+    if vocab < 1:
+        raise KernelArgumentError(f"{what}: an empty vocabulary")
+    n = temperature.numel()
+    for name, t, k in (("temperature", temperature, n), ("uniforms", uniforms, 2 * rows)):
+        if t.dtype is not torch.float32 or t.numel() < k or not t.is_contiguous():
+            raise KernelArgumentError(f"{what}: {name} must be contiguous float32 with at least {k} numbers")
+    tokens_at, drafted_at = _ints(what, "tokens", tokens, rows), _ints(what, "drafted", drafted, rows)
+    if tokens_at < drafted_at + 4 * rows and drafted_at < tokens_at + 4 * rows:
+        raise KernelArgumentError(f"{what}: tokens and drafted are two tensors")
+    _launch_on(device, what, "prb_verify_drafts", tokens_at, _ints(what, "accepted", accepted, n), logits.data_ptr(),
+               logits.stride(0), _ints(what, "row_start", row_start, n + 1), drafted_at,
+               None if draft_probs is None else draft_probs.data_ptr(),
+               0 if draft_probs is None else draft_probs.stride(0), uniforms.data_ptr(), temperature.data_ptr(), n, rows,
+               vocab, _status4(what, status))

@@ -1,0 +1,329 @@
+// Drafted tokens against the target's probabilities.
+//
+// A request brings n drafted tokens x_1 .. x_n and the target's logits of n + 1 rows: row i (from 0) says what comes
+// behind the i-th of them.  With p_i = softmax(row i / temperature), q_i what the draft drew x_{i+1} from and given
+// uniform numbers u_i, v_i in [0, 1):
+//   x_{i+1} stays while  u_i * q_i(x) < p_i(x)  and all before it stayed;
+//   the token behind the last that stays is drawn by v of its row: from max(p - q, 0), scaled to 1, where a token was
+//   refused (from p, should nothing be left), from p behind the last drafted one: the lowest index at which the
+//   running sum passes v times the whole.
+// Without probabilities of the draft q is 1 at the drafted token.  Temperature 0 or less: a token stays while it is the
+// largest logit (the lowest index among equals), and the largest logit follows.
+//
+// One launch; a cluster of eight CTAs takes a request, each an eighth of the vocabulary, and they meet through
+// distributed shared memory.  First all rows' maximum and sum of exponentials in 32 bits, one read of the logits from
+// memory, which is what bounds it: 64 requests of 5 rows of 50,257 are 64 MB.  Then the one row that is drawn from, in
+// 64 bits: the border between two tokens moves by the error of a running sum over the whole vocabulary, and in 32 bits
+// one draw in some hundred would fall on the other side.  The row comes from the L2, where the first pass left it.
+#include "common.cuh"
+#include "tcgen05.cuh"
+
+namespace {
+constexpr int PARTS = 8, THREADS = 512, WARPS = THREADS / 32;
+constexpr int MAX_ROWS = 32;
+
+struct VerifyArgs {
+    int* tokens;
+    int* accepted;
+    const float* logits;
+    long logits_stride;
+    const int* row_start;
+    const int* drafted;
+    const float* draft_probs;
+    long probs_stride;
+    const float* uniforms;
+    const float* temperature;
+    int n_requests, n_rows, vocab;
+    int* status;
+};
+
+struct Shared {
+    // a row's (maximum, its index, sum of exponentials) by warp, then of the CTA in place 0
+    float top[MAX_ROWS][WARPS], sum[MAX_ROWS][WARPS];
+    int index[MAX_ROWS][WARPS];
+    double part[WARPS], total;
+    int last[WARPS];             // the last token of a warp's run that has any weight
+    int last_all;
+};
+
+__device__ __forceinline__ uint32_t at_rank(const void* p, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(tc5::smem_u32(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float peer_f(const float* p, int rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at_rank(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ int peer_i(const int* p, int rank) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at_rank(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ double peer_d(const double* p, int rank) {
+    double v;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at_rank(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// (largest value, lowest index among equals)
+__device__ __forceinline__ void better(float& v, int& i, float w, int k) {
+    if (w > v || (w == v && k < i)) {
+        v = w;
+        i = k;
+    }
+}
+
+__global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS) verify_kernel(const VerifyArgs p) {
+    __shared__ Shared s;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int req = blockIdx.x / PARTS, rank = blockIdx.x % PARTS;
+    prb_grid_launch_dependents();
+    prb_grid_wait();
+    const int r0 = p.row_start[req], r1 = p.row_start[req + 1], rows = r1 - r0;
+    if (r0 < 0 || rows < 1 || rows > MAX_ROWS || r1 > p.n_rows) {         // (the whole cluster leaves)
+        if (threadIdx.x == 0 && rank == 0) {
+            prb_set_status(p.status, PRB_S_ROW_RANGE, r0, r1, p.n_rows);
+            p.accepted[req] = 0;
+        }
+        return;
+    }
+    const float t = p.temperature[req];
+    const bool greedy = !(t > 0.0f);
+    const float scale = greedy ? 1.0f : 1.4426950408889634f / t;
+    // this CTA's tokens, and each warp's run of them
+    const int each = (p.vocab + PARTS - 1) / PARTS;
+    const int lo = min(rank * each, p.vocab), hi = min(lo + each, p.vocab);
+
+    // ---------------------------------------------------------- every row: maximum, sum
+    for (int r = 0; r < rows; ++r) {
+        const float* x = p.logits + (long)(r0 + r) * p.logits_stride;
+        float top = -INFINITY, sum = 0.0f;
+        int index = 0x7fffffff;
+        auto take = [&](const float (&v)[4], const int (&k)[4], int n) {
+            float now = top;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < n && (v[i] > now || (index == 0x7fffffff && i == 0))) {
+                    now = v[i];
+                    index = k[i];
+                }
+            if (!greedy) {
+                const float ref = now == -INFINITY ? 0.0f : now;
+                sum *= exp2f((top - ref) * scale);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i < n) sum += exp2f((v[i] - ref) * scale);
+            }
+            top = now;
+        };
+        // (a thread's tokens go up, so the first of equals is kept)
+        for (int i = lo + threadIdx.x; i < hi; i += 4 * THREADS) {
+            float v[4];
+            int k[4], n = 0;
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+                k[z] = i + z * THREADS;
+                v[z] = k[z] < hi ? x[k[z]] : 0.0f;
+                n += k[z] < hi;
+            }
+            take(v, k, n);
+        }
+        // the warp's lanes
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const float v = __shfl_xor_sync(0xffffffffu, top, o), w = __shfl_xor_sync(0xffffffffu, sum, o);
+            const int k = __shfl_xor_sync(0xffffffffu, index, o);
+            const float was = top;
+            better(top, index, v, k);
+            if (!greedy) {
+                const float ref = top == -INFINITY ? 0.0f : top;
+                sum = sum * exp2f((was - ref) * scale) + w * exp2f((v - ref) * scale);
+            }
+        }
+        if (lane == 0) {
+            s.top[r][warp] = top;
+            s.sum[r][warp] = sum;
+            s.index[r][warp] = index;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < rows) {
+        const int r = threadIdx.x;
+        float top = s.top[r][0], sum = s.sum[r][0];
+        int index = s.index[r][0];
+        for (int w = 1; w < WARPS; ++w) {
+            const float was = top, v = s.top[r][w];
+            better(top, index, v, s.index[r][w]);
+            if (!greedy) {
+                const float ref = top == -INFINITY ? 0.0f : top;
+                sum = sum * exp2f((was - ref) * scale) + s.sum[r][w] * exp2f((v - ref) * scale);
+            }
+        }
+        s.top[r][0] = top;
+        s.sum[r][0] = sum;
+        s.index[r][0] = index;
+    }
+    cluster_sync_all();
+
+    // -------------------------------- who stays: lane i looks at row i, every warp by itself
+    float top = -INFINITY;
+    int best = 0x7fffffff;
+    bool stays = false;
+    if (lane < rows) {
+        float part[PARTS], sum = 0.0f;
+#pragma unroll
+        for (int z = 0; z < PARTS; ++z) {
+            part[z] = peer_f(&s.top[lane][0], z);
+            better(top, best, part[z], peer_i(&s.index[lane][0], z));
+        }
+        const float ref = top == -INFINITY ? 0.0f : top;
+        if (!greedy) {
+#pragma unroll
+            for (int z = 0; z < PARTS; ++z) sum += peer_f(&s.sum[lane][0], z) * exp2f((part[z] - ref) * scale);
+            if (!(fabsf(top) < INFINITY && sum > 0.0f && sum < INFINITY) && rank == 0 && warp == 0)
+                prb_set_status(p.status, PRB_S_LOGITS, r0 + lane, req, 0);
+        } else if (!(fabsf(top) < INFINITY) && rank == 0 && warp == 0) {
+            prb_set_status(p.status, PRB_S_LOGITS, r0 + lane, req, 0);
+        }
+        if (lane + 1 < rows) {
+            const int x = p.drafted[r0 + lane];
+            if (x < 0 || x >= p.vocab) {
+                if (rank == 0 && warp == 0) prb_set_status(p.status, PRB_S_TOKEN_RANGE, r0 + lane, x, p.vocab);
+            } else if (greedy) {
+                stays = x == best;
+            } else {
+                const double mine = exp(((double)p.logits[(long)(r0 + lane) * p.logits_stride + x] - (double)ref) / (double)t);
+                const double theirs = p.draft_probs ? (double)p.draft_probs[(long)(r0 + lane) * p.probs_stride + x] : 1.0;
+                stays = (double)p.uniforms[2 * (r0 + lane)] * theirs * (double)sum < mine;
+            }
+        }
+    }
+    const int kept = __ffs(~__ballot_sync(0xffffffffu, stays)) - 1;       // (row rows - 1 never stays)
+    const int row = r0 + kept;
+    const bool refused = kept + 1 < rows;
+    int chosen = __shfl_sync(0xffffffffu, best, kept);
+    top = __shfl_sync(0xffffffffu, top, kept);
+    if (chosen >= p.vocab) chosen = 0;
+
+    if (!greedy && fabsf(top) < INFINITY) {
+        // ------------------------------------------------- the row that is drawn from, in 64 bits
+        const float* x = p.logits + (long)row * p.logits_stride;
+        const float* q = refused && p.draft_probs ? p.draft_probs + (long)row * p.probs_stride : nullptr;
+        const int gone = refused && !p.draft_probs ? p.drafted[row] : -1;
+        const double inverse = 1.0 / (double)t;
+        const int run = (hi - lo + WARPS - 1) / WARPS;
+        const int w0 = min(lo + warp * run, hi), w1 = min(w0 + run, hi);
+        // the CTA's sum, then all CTAs'
+        auto meet = [&](double v) -> double {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            cluster_sync_all();                                           // (the last meeting's sums are read)
+            if (lane == 0) s.part[warp] = v;
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                double a = 0.0;
+                for (int w = 0; w < WARPS; ++w) a += s.part[w];
+                s.total = a;
+            }
+            cluster_sync_all();
+            double all = 0.0;
+            for (int z = 0; z < PARTS; ++z) all += peer_d(&s.total, z);
+            return all;
+        };
+        double z = 0.0;
+        for (int i = w0 + lane; i < w1; i += 32) z += exp(((double)x[i] - (double)top) * inverse);
+        z = meet(z);
+        auto weight = [&](int i, bool less) -> double {
+            const double w = exp(((double)x[i] - (double)top) * inverse) / z;
+            if (!less) return w;
+            if (q != nullptr) return fmax(w - (double)q[i], 0.0);
+            return i == gone ? 0.0 : w;
+        };
+        bool less = refused;
+        double whole = 0.0;
+        for (int go = 0; go < 2; ++go) {
+            double v = 0.0;
+            for (int i = w0 + lane; i < w1; i += 32) v += weight(i, less);
+            whole = meet(v);
+            if (whole > 0.0 || !less) break;
+            less = false;                                                 // nothing left: the target's own
+        }
+        const double want = (double)p.uniforms[2 * row + 1] * whole;
+        // the CTA whose sums pass it, else the last that has any weight
+        double before = 0.0;
+        int owner = -1, final_owner = 0;
+        double owner_before = 0.0;
+        for (int c = 0; c < PARTS; ++c) {
+            const double v = peer_d(&s.total, c);
+            if (v > 0.0) final_owner = c;
+            if (owner < 0 && before + v > want) {
+                owner = c;
+                owner_before = before;
+            }
+            before += v;
+        }
+        const bool passes = owner >= 0;
+        if (!passes) owner = final_owner;
+        if (owner == rank) {
+            double b = owner_before;
+            int mine = -1, final_mine = 0;
+            double mine_before = 0.0;
+            for (int w = 0; w < WARPS; ++w) {
+                const double v = s.part[w];
+                if (v > 0.0) final_mine = w;
+                if (mine < 0 && passes && b + v > want) {
+                    mine = w;
+                    mine_before = b;
+                }
+                b += v;
+            }
+            const bool inside = mine >= 0;
+            if (!inside) mine = final_mine;
+            if (mine == warp) {
+                double sum = mine_before;
+                int found = -1, final_token = w0;
+                for (int i0 = w0; i0 < w1 && found < 0; i0 += 32) {
+                    const int i = i0 + lane;
+                    const double w = i < w1 ? weight(i, less) : 0.0;
+                    double up = w;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const double v = __shfl_up_sync(0xffffffffu, up, o);
+                        if (lane >= o) up += v;
+                    }
+                    const unsigned over = __ballot_sync(0xffffffffu, inside && w > 0.0 && sum + up > want);
+                    const unsigned any = __ballot_sync(0xffffffffu, w > 0.0);
+                    if (any) final_token = i0 + 31 - __clz(any);
+                    if (over) found = i0 + __ffs(over) - 1;
+                    sum += __shfl_sync(0xffffffffu, up, 31);
+                }
+                if (lane == 0) p.tokens[row] = found >= 0 ? found : final_token;
+            }
+        }
+    } else if (rank == 0 && threadIdx.x == 0) {
+        p.tokens[row] = chosen;
+    }
+    if (rank == 0) {
+        for (int r = threadIdx.x; r < rows; r += THREADS)
+            if (r != kept) p.tokens[r0 + r] = r < kept ? p.drafted[r0 + r] : -1;
+        if (threadIdx.x == 0) p.accepted[req] = kept;
+    }
+    cluster_sync_all();                                                   // nobody leaves while its sums may be read
+}
+}  // namespace
+
+PRB_API int prb_verify_drafts(int* tokens, int* accepted, const float* logits, long logits_stride, const int* row_start,
+                              const int* drafted, const float* draft_probs, long probs_stride, const float* uniforms,
+                              const float* temperature, int n_requests, int n_rows, int vocab, int* status,
+                              cudaStream_t stream) {
+    if (n_requests <= 0 || n_rows <= 0) return 0;
+    if (vocab <= 0 || n_requests > 0x7fffffff / PARTS) return PRB_E_SIZE;
+    const VerifyArgs a{tokens, accepted, logits, logits_stride, row_start, drafted, draft_probs, probs_stride, uniforms,
+                       temperature, n_requests, n_rows, vocab, status};
+    const cudaError_t e = prb_launch_dependent(verify_kernel, dim3((unsigned)n_requests * PARTS), dim3(THREADS), 0, stream, a);
+    return e == cudaSuccess ? 0 : (int)e;
+}

@@ -1,0 +1,180 @@
+"""What the entry points of the 4-bit cache, the step tables and the drafted tokens refuse before anything is launched,
+and the plain statement that their kernels are tested against."""
+import math
+
+import pytest
+import torch
+
+import plain_cache4 as plain
+
+
+def test_packing_and_unpacking():
+    g = torch.Generator().manual_seed(0)
+    for d in (16, 48, 64, 80, 112, 128):
+        x = torch.randn(3, 2, 16, d, generator=g)
+        q = plain.quantize(x)
+        tiles = plain.pack(*q)
+        assert tiles.shape == (3, 2, plain.tile_bytes(16, d))
+        for a, b in zip(plain.unpack(tiles, 16, d), q):
+            assert torch.equal(a.double(), b.double())
+
+
+def test_a_number_comes_back_within_its_roundings():
+    """Half a step, and where step and middle were rounded (2^-8 of each) at the ends of the range."""
+    x = torch.randn(50, 64, generator=torch.Generator().manual_seed(1)).double()
+    codes, step, middle = plain.quantize(x)
+    a, b = plain.values(codes, step, middle)
+    wide = step.repeat_interleave(32, -1)
+    err = (a + b - x).abs()
+    assert bool((err <= wide * (0.5 + 8 * 2.0 ** -8) + middle.abs().repeat_interleave(32, -1) * 2.0 ** -8).all())
+
+
+def test_values_on_the_border_of_two_codes_go_to_the_even_one():
+    x = torch.zeros(1, 32)
+    x[0, 0], x[0, 1], x[0, 2], x[0, 3], x[0, 4] = -8.0, 7.0, 0.5, 1.5, -2.5
+    codes, step, middle = plain.quantize(x)
+    assert step.item() == 1.0 and middle.item() == 0.0
+    assert codes[0, :5].tolist() == [0.0, 15.0, 8.0, 10.0, 6.0]
+
+
+def test_the_plain_attention_is_a_softmax_over_what_the_cache_stands_for():
+    g = torch.Generator().manual_seed(2)
+    kt, vt = (plain.pack(*plain.quantize(torch.randn(3, 1, 16, 32, generator=g))) for _ in range(2))
+    q = torch.randn(1, 64, generator=g)
+    out, _terms = plain.attention(q, kt, vt, [[2, 0]], [20], [0], 2, 32, 16, 0.3, 5)
+    read = lambda t: sum(plain.values(*plain.unpack(t[[2, 0]], 16, 32))).transpose(0, 1).flatten(1, 2)[0, 16:21]  # noqa: E731
+    k, v = read(kt), read(vt)
+    for h in range(2):
+        w = torch.exp(0.3 * (k @ q[0, 32 * h:32 * h + 32].double()))
+        assert torch.allclose(out[0, 32 * h:32 * h + 32], (w @ v) / w.sum(), atol=1e-12)
+
+
+def test_the_plain_verification_follows_the_rule():
+    logits = torch.log(torch.tensor([[0.5, 0.3, 0.2], [0.1, 0.1, 0.8]]))
+    q = torch.tensor([[0.2, 0.7, 0.1], [0.3, 0.3, 0.4]])
+    # stays: 0.4 * 0.7 < 0.3; behind it the last row's own draw
+    assert plain.verify(logits, [0, 2], [1, 0], [[0.4, 0.9], [0.0, 0.15]], [1.0], q) == ([1, 1], [1])
+    # refused: 0.5 * 0.7 > 0.3; the rest of p - q is (0.3, 0, 0.1)
+    assert plain.verify(logits, [0, 2], [1, 0], [[0.5, 0.7], [0.0, 0.0]], [1.0], q) == ([0, -1], [0])
+    assert plain.verify(logits, [0, 2], [1, 0], [[0.5, 0.8], [0.0, 0.0]], [1.0], q) == ([2, -1], [0])
+    assert plain.verify(logits, [0, 2], [0, 0], [[0.5, 0.8], [0.0, 0.0]], [0.0]) == ([0, 2], [1])
+
+
+# ------------------------------------------------------------------------------------ refusals
+# (shapes and types are looked at before the library is asked for anything: no device is needed to be refused)
+class _FakeCuda(torch.Tensor):
+    """A tensor that says it lies on the GPU; nothing may get as far as its memory."""
+    def get_device(self):
+        return 0
+
+
+def fake(*shape, dtype=torch.int32):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(_FakeCuda)
+
+
+@pytest.fixture
+def ops(monkeypatch):
+    from pretrained_rstr_b200.csrc import ops as module
+
+    def launched(*_a, **_k):
+        raise AssertionError("a refused call reached the library")
+    monkeypatch.setattr(module, "lib", launched)
+    return module
+
+
+def _append_args(**kw):
+    a = dict(k_tiles=fake(4, 2, plain.tile_bytes(16, 32), dtype=torch.uint8),
+             v_tiles=fake(4, 2, plain.tile_bytes(16, 32), dtype=torch.uint8), k=fake(5, 64, dtype=torch.bfloat16),
+             v=fake(5, 64, dtype=torch.bfloat16), slots=fake(5), n_tokens=5, head_dim=32, page_size=16, status=fake(4))
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(head_dim=24), "multiples of 16"), (dict(head_dim=144), "up to 128"), (dict(page_size=8), "pages"),
+    (dict(k=fake(5, 60, dtype=torch.bfloat16)), "k must be"), (dict(v=fake(4, 64, dtype=torch.bfloat16)), "v must be"),
+    (dict(k=fake(5, 64, dtype=torch.float32)), "differ in type"), (dict(k=fake(5, 64, dtype=torch.float16)), "not supported"),
+    (dict(slots=fake(4)), "slots"), (dict(slots=fake(5, dtype=torch.int64)), "slots"),
+    (dict(k_tiles=fake(4, 2, 100, dtype=torch.uint8)), "k_tiles"), (dict(status=fake(2)), "status"),
+    (dict(v_tiles=fake(3, 2, plain.tile_bytes(16, 32), dtype=torch.uint8)), "differ in shape"),
+    (dict(k=torch.zeros(5, 64, dtype=torch.bfloat16)), "not on a CUDA device"),
+    (dict(n_tokens=-1), "n_tokens")])
+def test_rows_refused(ops, change, word):
+    with pytest.raises(ops.KernelArgumentError, match=word):
+        ops.kv_append_4bit(**_append_args(**change))
+    back = _append_args(**change)
+    back["k_out"], back["v_out"] = back.pop("k"), back.pop("v")
+    with pytest.raises(ops.KernelArgumentError, match=word.replace("k must", "k_out must").replace("v must", "v_out must")):
+        ops.kv_read_4bit(**back)
+
+
+def _attention_args(**kw):
+    a = dict(out=fake(6, 128, dtype=torch.bfloat16), q=fake(6, 128, dtype=torch.bfloat16),
+             k_tiles=fake(4, 2, plain.tile_bytes(16, 32), dtype=torch.uint8),
+             v_tiles=fake(4, 2, plain.tile_bytes(16, 32), dtype=torch.uint8), block_table=fake(3, 7), positions=fake(6),
+             tile_req=fake(2), tile_row0=fake(2), tile_rows=fake(2), tile_most=4, n_heads=4, head_dim=32, page_size=16,
+             scale=0.1, window=None, max_context=50, status=fake(4))
+    a.update(kw)
+    return a
+
+
+_Q = fake(6, 128, dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(n_heads=3), "multiple"), (dict(n_heads=0), "multiple"), (dict(q=fake(6, 120, dtype=torch.bfloat16)), "q must be"),
+    (dict(out=fake(5, 128, dtype=torch.bfloat16)), "out must be"), (dict(out=fake(6, 128, dtype=torch.float32)), "differ in type"),
+    (dict(positions=fake(5)), "positions"), (dict(tile_rows=fake(1)), "tile_rows"), (dict(window=0), "window"),
+    (dict(window=-3), "window"), (dict(tile_count=fake(0)), "tile_count"), (dict(block_table=fake(7)), "block_table"),
+    (dict(block_table=fake(3, 7, dtype=torch.int64)), "block_table"), (dict(q=_Q, out=_Q), "out must not be q"),
+    (dict(tile_most=0), "tile_most"), (dict(max_context=0), "max_context"), (dict(parts=9), "parts"),
+    (dict(scale=math.nan), "scale"), (dict(head_dim=40), "multiples of 16")])
+def test_attention_refused(ops, change, word):
+    with pytest.raises(ops.KernelArgumentError, match=word):
+        ops.attention_4bit(**_attention_args(**change))
+
+
+def _table_args(**kw):
+    a = dict(rows=fake(3), held=fake(3), brought=fake(3), tables=fake(5, 4), page_size=16, q_start=fake(4), kv_len=fake(3),
+             positions=fake(9), seq_of_token=fake(9), slots=fake(9), block_table=fake(3, 4), status=fake(4),
+             free_pages=fake(2), free_start=fake(1), free_next=fake(1))
+    a.update(kw)
+    return a
+
+
+_ONE = fake(1)
+_T = fake(5, 4)
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(rows=fake(2)), "rows"), (dict(q_start=fake(3)), "q_start"), (dict(slots=fake(8)), "slots"),
+    (dict(block_table=fake(2, 4)), "block_table"), (dict(block_table=fake(3, 5)), "block_table"),
+    (dict(tables=fake(4)), "tables"), (dict(page_size=0), "page_size"), (dict(held=fake(0)), "requests"),
+    (dict(held=fake(4097)), "requests"), (dict(free_start=None), "free_start"), (dict(free_next=None), "free_next"),
+    (dict(free_start=_ONE, free_next=_ONE), "free_next must not"), (dict(brought=fake(3, dtype=torch.int64)), "brought"),
+    (dict(tables=_T, block_table=_T), "two tensors")])
+def test_tables_refused(ops, change, word):
+    with pytest.raises(ops.KernelArgumentError, match=word):
+        ops.step_tables(**_table_args(**change))
+
+
+def _verify_args(**kw):
+    f = torch.float32
+    a = dict(tokens=fake(6), accepted=fake(2), logits=fake(6, 10, dtype=f), row_start=fake(3), drafted=fake(6),
+             uniforms=fake(6, 2, dtype=f), temperature=fake(2, dtype=f), status=fake(4), draft_probs=fake(6, 10, dtype=f))
+    a.update(kw)
+    return a
+
+
+_W = fake(6)
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(logits=fake(6, 10, dtype=torch.bfloat16)), "logits"), (dict(draft_probs=fake(6, 9, dtype=torch.float32)), "differ in shape"),
+    (dict(uniforms=fake(5, 2, dtype=torch.float32)), "uniforms"), (dict(row_start=fake(2)), "row_start"),
+    (dict(accepted=fake(1)), "accepted"), (dict(temperature=fake(2, dtype=torch.float64)), "temperature"),
+    (dict(logits=fake(6, 0, dtype=torch.float32), draft_probs=None), "vocabulary"), (dict(drafted=fake(6, dtype=torch.int64)), "drafted"),
+    (dict(tokens=_W, drafted=_W), "two tensors"), (dict(tokens=fake(5)), "tokens")])
+def test_verification_refused(ops, change, word):
+    with pytest.raises(ops.KernelArgumentError, match=word):
+        ops.verify_drafts(**_verify_args(**change))
