@@ -11,15 +11,21 @@
 // as probabilities are rounded before any such product).  float32 queries, and then p * step, go as the sum of
 // three bfloat16 numbers (24 bits), which makes three products of 32-bit exactness.
 //
-// What bounds it: the bytes of the cache where there is one row a key/value head, the instructions that turn words of
-// codes into operands beside them (11 a word of 8 codes), the products from some rows on.
+// Keys and values are the left operand (16 keys x 16 channels, 16 channels x 16 keys), queries and probabilities the
+// right one (8 rows a product): one decoded token with a key/value head of its own wastes 7 of 8 columns rather than
+// 15 of 16 rows, a thread looks after the steps and middles of 2 keys in 16 rather than 4, and half as many products do.  The
+// scores' accumulator has keys along lanes where the probabilities' operand has rows there: a transposing move of an
+// 8 x 8 block of the rounded numbers (movmatrix) turns one into the other.
 //
-// One CTA of four warps takes up to 16 rows (8 in the LOW form; a row is a token and one of the heads that share keys
-// and values) of one tile for one key/value head, or one of S parts of their keys; the parts are a cluster, whose
-// CTAs meet through distributed shared memory, so there is no workspace and no counter, and parts are added in the
-// keys' order whatever came first.  Each warp takes every fourth stage of SK keys and keeps two stages of its own in
-// flight (bulk copies, no multicast, of whole tiles where a page is a stage).  Nothing is shared between warps until
-// the end.
+// What bounds it: the instructions that turn words of codes into operands and scale them; then the bytes of the cache.
+// With bfloat16 queries the 8 stays in the codes of the keys (128 + c is what the bits of a code make without an
+// addition) and goes with the middle: q . (128 + c) is off by 2^-24 of 136 sums of |q|, which is nothing there.
+//
+// One CTA takes up to 8 QN rows (a row is a token and one of the heads that share keys and values) of one tile for one
+// key/value head, or one of the parts of their keys; the parts are a cluster, whose CTAs meet through distributed
+// shared memory, so there is no workspace and no counter, and parts are added in the keys' order whatever came first.
+// Each of its warps takes every nth stage of SK keys and keeps two stages of its own in flight (bulk copies, no
+// multicast, of whole tiles where a page is a stage).  Nothing is shared between warps until the end.
 #pragma once
 #include "cache4.cuh"
 #include "tcgen05.cuh"
@@ -27,12 +33,12 @@
 namespace attn4 {
 using namespace tc5;
 
-constexpr int WARPS = 4, THREADS = WARPS * 32;
+constexpr int MAX_WARPS = 4;
 constexpr int STAGES = 2;                  // ring buffers of a warp
 constexpr int MAX_PARTS = 8;               // CTAs of a cluster (portable)
 
-// keys of a stage: 64, or 32 where four groups would make a warp's two buffers larger than an SM likes
-__host__ __device__ constexpr int stage_keys(int ng) { return ng <= 2 ? 64 : 32; }
+// keys of a stage: 64, or 32 where a warp's buffers or its scores would grow too large
+__host__ __device__ constexpr int stage_keys(int ng, int qn) { return ng <= 2 && qn <= 2 ? 64 : 32; }
 
 struct Args {
     void* out;
@@ -49,7 +55,7 @@ struct Args {
     const int* tile_count;                 // null: every tile of the launch
     int n_tokens;                          // rows of q and out
     int n_requests;                        // rows of the block table
-    int n_tiles, subs, parts;
+    int n_tiles, subs, parts, warps;
     int heads, kv_heads, hpg;              // hpg: query heads per key/value head
     int head_dim, page_size, piece;        // piece: keys that lie together in a page and in a stage
     int max_pages, num_pages;
@@ -67,17 +73,24 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 }
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                  "{%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Codes i and i + 4 of a word, less 8, as two bfloat16 numbers: 0x4300 | c is 128 + c.
-__device__ __forceinline__ uint32_t code_pair(uint32_t word, int i) {
+// Codes i and i + 4 of a word as two bfloat16 numbers: 0x4300 | c is 128 + c; less 136 if CENTRED.
+template <bool CENTRED> __device__ __forceinline__ uint32_t code_pair(uint32_t word, int i) {
     const uint32_t u = ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    if (!CENTRED) return u;
     const __nv_bfloat162 off = __floats2bfloat162_rn(136.0f, 136.0f);
     const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), off);
     return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Row r, columns 2 c and 2 c + 1 of an 8 x 8 block in lane 4 r + c -> the same of its transpose.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -110,29 +123,33 @@ template <int PIECES> __device__ __forceinline__ void split2(float x, float y, u
     }
 }
 
-template <int NG> struct Layout {
-    static constexpr int SK = stage_keys(NG);
+template <int NG, int QN> struct Layout {
+    static constexpr int SK = stage_keys(NG, QN), ROWS = 8 * QN;
+    static constexpr int DP = NG * 32, PART = DP + 2;         // floats a row of a partial state: values, maximum, sum
     static constexpr int KIND = SK * (16 * NG + 4 * NG);      // most bytes of a stage's keys (and of its values)
     static constexpr int STAGE = 2 * KIND;
-    static constexpr int RING = WARPS * STAGES * STAGE;
-    static constexpr int BARS = WARPS * STAGES * 8;
+    // a warp's ring, which takes its state in the end
+    static constexpr int STATE = (ROWS * PART * 4 + 15) / 16 * 16;
+    static constexpr int WARP = STAGES * STAGE > STATE ? STAGES * STAGE : STATE;
+    static constexpr int bytes(int warps) { return warps * (WARP + STAGES * 8) + 16; }
 };
 
-template <int NG, bool LOW, typename T>
-__global__ void __launch_bounds__(THREADS) attention_4bit_kernel(const Args p) {
-    using L = Layout<NG>;
-    constexpr int SK = L::SK, ROWS = LOW ? 8 : 16, NT = SK / 8, RH = LOW ? 1 : 2;
+// FAST: the head size is 32 NG and a stage lies in one page, so that every offset is known here.
+template <int NG, int QN, typename T, bool FAST>
+__global__ void __launch_bounds__(MAX_WARPS * 32, QN == 1 ? (NG <= 2 ? 4 : 3) : 2) attention_4bit_kernel(const Args p) {
+    using L = Layout<NG, QN>;
+    constexpr int SK = L::SK, ROWS = L::ROWS, NC = SK / 16, DP = L::DP, PART = L::PART;
     constexpr int PIECES = sizeof(T) == 4 ? 3 : 1;
-    constexpr int DP = NG * 32, PART = DP + 2;                // floats a row of a partial state: values, maximum, sum
+    constexpr bool EXACT = PIECES == 3;                       // codes less 8 in the keys' products too
     extern __shared__ __align__(128) uint8_t smem[];
-    static_assert(ROWS * PART * 4 <= STAGES * L::STAGE, "a warp's state fits its own ring");
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::RING);
-    volatile int* failed = reinterpret_cast<volatile int*>(smem + L::RING + L::BARS);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + p.warps * L::WARP);
+    volatile int* failed = reinterpret_cast<volatile int*>(bars + p.warps * STAGES);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n = lane >> 2, j = lane & 3;
+    const int threads = p.warps * 32;
     prb_grid_launch_dependents();
-    if (threadIdx.x < WARPS * STAGES) mbar_init(smem_u32(&bars[threadIdx.x]), 1);
+    if (threadIdx.x < p.warps * STAGES) mbar_init(smem_u32(&bars[threadIdx.x]), 1);
     if (threadIdx.x == 0) *failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -164,21 +181,77 @@ __global__ void __launch_bounds__(THREADS) attention_4bit_kernel(const Args p) {
     const int my_hi = blk_lo + (int)((long)n_blk * (rank + 1) / p.parts);
     const int* table = p.block_table + (size_t)req * p.max_pages;
 
+    // ------------------------------------------------------------------------ stages
+    const uint32_t ring = smem_u32(smem) + warp * L::WARP;
+    const uint8_t* ring_p = smem + warp * L::WARP;
+    const uint32_t bar0 = smem_u32(&bars[warp * STAGES]);
+    const int head_dim = FAST ? DP : p.head_dim;
+    const int piece = FAST ? SK : p.piece;                    // 16, 32 or 64
+    const int pieces = SK / piece, piece_log = __popc(piece - 1);
+    const int piece_bytes = piece * (head_dim / 2 + 4 * NG);
+    const int codes_of_page = p.page_size * (head_dim / 2);
+    // Lane i looks after piece i of a stage: its page, ahead of time, and its copies.
+    auto page_of = [&](int blk) -> int {
+        const int key = blk * SK + lane * piece;
+        if (blk >= my_hi || lane >= pieces || key > pos_hi || key + piece <= key_lo) return -2;    // nothing to fetch
+        return table[key / p.page_size];
+    };
+    auto request = [&](int blk, int st, int page) {
+        bool fetch = page != -2;
+        if (fetch && (page < 0 || page >= p.num_pages)) {
+            // (recorded; the stage keeps what it held, and the tile's result is not to be used)
+            prb_set_status(p.status, PRB_S_PAGE_RANGE, row0, blk * SK + lane * piece, page);
+            fetch = false;
+        }
+        const unsigned who = __ballot_sync(0xffffffffu, fetch);
+        const uint32_t bar = bar0 + st * 8;
+        if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(who) * 2 * piece_bytes));
+        __syncwarp();
+        if (!fetch) return;
+        const int at = (blk * SK + lane * piece) % p.page_size;
+#pragma unroll
+        for (int kind = 0; kind < 2; ++kind) {
+            const uint8_t* src = (kind ? p.v_tiles : p.k_tiles) + ((size_t)page * p.kv_heads + hk) * (size_t)p.tile_bytes;
+            uint32_t dst = ring + st * L::STAGE + kind * L::KIND + lane * piece_bytes;
+            if (piece == p.page_size) {
+                bulk_load(dst, src, piece_bytes, bar);
+            } else {
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const int row = min(16, (head_dim - g * 32) / 2);
+                    bulk_load(dst, src + g * p.page_size * 16 + at * row, piece * row, bar);
+                    dst += piece * row;
+                }
+                bulk_load(dst, src + codes_of_page + at * NG * 4, piece * NG * 4, bar);
+            }
+        }
+    };
+#pragma unroll
+    for (int st = 0; st < STAGES; ++st) {
+        const int blk = my_lo + warp + st * p.warps;
+        if (blk < my_hi) request(blk, st, page_of(blk));
+    }
+    int ahead = page_of(my_lo + warp + STAGES * p.warps);
+
     // ---------------------------------------------------------------------- queries
     // Channel order of the reduction: thread j of a quad has channels 8 j + (i, i + 4), the codes that one shift and
     // one mask take from word j.
-    uint32_t qa[NG][2][PIECES][2 * RH];                       // [group][half of the reduction][piece][operand]
-    float qsum[NG][RH];
+    uint32_t qb[QN][NG][2][PIECES][2];                        // [rows][group][half of the reduction][piece][operand]
+    float qsum[QN][NG][2];                                    // of rows 2 j and 2 j + 1
+    int pos[QN][2];
 #pragma unroll
-    for (int r = 0; r < RH; ++r) {
-        const int row = n + 8 * r, at = first + min(row, rows - 1);
+    for (int z = 0; z < QN; ++z) {
+        const int row = n + 8 * z, at = first + min(row, rows - 1);
         const int tk = at / p.hpg, h = hk * p.hpg + at - tk * p.hpg;
-        const T* src = reinterpret_cast<const T*>(p.q) + (long)(row0 + tk) * p.q_stride + (long)h * p.head_dim;
+        const int here = pos0 + tk;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) pos[z][e] = __shfl_sync(0xffffffffu, here, (2 * j + e) * 4);
+        const T* src = reinterpret_cast<const T*>(p.q) + (long)(row0 + tk) * p.q_stride + (long)h * head_dim;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             const int c0 = g * 32 + j * 8;
             float x[8];
-            if (row < rows && c0 < p.head_dim) {
+            if (row < rows && c0 < head_dim) {
                 if (p.wide) {
                     if (sizeof(T) == 2) {
                         const uint4 w = *reinterpret_cast<const uint4*>(src + c0);
@@ -207,92 +280,42 @@ __global__ void __launch_bounds__(THREADS) attention_4bit_kernel(const Args p) {
             for (int i = 0; i < 8; ++i) sum += x[i];
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            qsum[g][r] = sum;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) qsum[z][g][e] = __shfl_sync(0xffffffffu, sum, (2 * j + e) * 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 uint32_t w[PIECES];
                 split2<PIECES>(x[i], x[i + 4], w);
 #pragma unroll
-                for (int z = 0; z < PIECES; ++z) qa[g][i >> 1][z][(i & 1) * RH + r] = w[z];
+                for (int y = 0; y < PIECES; ++y) qb[z][g][i >> 1][y][i & 1] = w[y];
             }
         }
     }
 
-    // ------------------------------------------------------------------------ stages
-    const uint32_t ring = smem_u32(smem) + warp * STAGES * L::STAGE;
-    const uint8_t* ring_p = smem + warp * STAGES * L::STAGE;
-    const uint32_t bar0 = smem_u32(&bars[warp * STAGES]);
-    const int pieces = SK / p.piece;
-    const int piece_bytes = p.piece * (p.head_dim / 2 + 4 * NG);
-    const int codes_of_page = p.page_size * (p.head_dim / 2);
-    const bool whole = p.piece == p.page_size;
-    // Lane i looks after piece i of a stage: its page, ahead of time, and its copies.
-    auto page_of = [&](int blk) -> int {
-        const int key = blk * SK + lane * p.piece;
-        if (blk >= my_hi || lane >= pieces || key > pos_hi || key + p.piece <= key_lo) return -2;    // nothing to fetch
-        return table[key / p.page_size];
-    };
-    auto request = [&](int blk, int st, int page) {
-        bool fetch = page != -2;
-        if (fetch && (page < 0 || page >= p.num_pages)) {
-            // (recorded; the stage keeps what it held, and the tile's result is not to be used)
-            prb_set_status(p.status, PRB_S_PAGE_RANGE, row0, blk * SK + lane * p.piece, page);
-            fetch = false;
-        }
-        const unsigned who = __ballot_sync(0xffffffffu, fetch);
-        const uint32_t bar = bar0 + st * 8;
-        if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(who) * 2 * piece_bytes));
-        __syncwarp();
-        if (!fetch) return;
-        const int at = (blk * SK + lane * p.piece) % p.page_size;
+    // results [rows][group][16 of its channels]: channels (2 i, 2 i + 1 of the thread's four) x rows (2 j, 2 j + 1)
+    float o[QN][NG][2][4];
+    float mid[QN][NG][2], m[QN][2], l[QN][2];
 #pragma unroll
-        for (int kind = 0; kind < 2; ++kind) {
-            const uint8_t* src = (kind ? p.v_tiles : p.k_tiles) + ((size_t)page * p.kv_heads + hk) * (size_t)p.tile_bytes;
-            uint32_t dst = ring + st * L::STAGE + kind * L::KIND + lane * piece_bytes;
-            if (whole) {
-                bulk_load(dst, src, piece_bytes, bar);
-            } else {
+    for (int z = 0; z < QN; ++z)
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const int row = min(16, (p.head_dim - g * 32) / 2);
-                    bulk_load(dst, src + g * p.page_size * 16 + at * row, p.piece * row, bar);
-                    dst += p.piece * row;
-                }
-                bulk_load(dst, src + codes_of_page + at * NG * 4, p.piece * NG * 4, bar);
+        for (int e = 0; e < 2; ++e) {
+            m[z][e] = -INFINITY;
+            l[z][e] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                mid[z][g][e] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[z][g][e][i] = 0.0f;
             }
         }
-    };
-
-    float o[NG][4][4];
-    float mid[NG][RH], m[RH], l[RH];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[g][i][e] = 0.0f;
-#pragma unroll
-        for (int r = 0; r < RH; ++r) mid[g][r] = 0.0f;
-    }
-#pragma unroll
-    for (int r = 0; r < RH; ++r) {
-        m[r] = -INFINITY;
-        l[r] = 0.0f;
-    }
     const float sl2 = p.scale * 1.4426950408889634f;          // scores are handled in log2 units
     // (the short last group's rows are 8 bytes apart; its words 2 and 3 do not exist: words 0 and 1 stand in, against
     // queries of zero and for channels that are not stored)
-    const bool short_last = p.head_dim % 32 != 0;
+    const bool short_last = !FAST && head_dim % 32 != 0;
 
-#pragma unroll
-    for (int st = 0; st < STAGES; ++st) {
-        const int blk = my_lo + warp + st * WARPS;
-        if (blk < my_hi) request(blk, st, page_of(blk));
-    }
-    int ahead = page_of(my_lo + warp + STAGES * WARPS);
     bool alive = true;
     int it = 0;
-    for (int blk = my_lo + warp; blk < my_hi; blk += WARPS, ++it) {
+    for (int blk = my_lo + warp; blk < my_hi; blk += p.warps, ++it) {
         const int st = it % STAGES;
         alive = mbar_wait_warp(bar0 + st * 8, (it / STAGES) & 1, failed);
         if (!alive) {
@@ -303,163 +326,175 @@ __global__ void __launch_bounds__(THREADS) attention_4bit_kernel(const Args p) {
         const uint8_t* vs = ks + L::KIND;
         const int key0 = blk * SK;
         const bool masked = key0 + SK - 1 > pos_lo || (p.window > 0 && key0 <= pos_hi - p.window);
-        // ---- scores
-        float s[NT][2 * RH];
+        // ---- scores of keys n and n + 8 of every 16
+        float s[NC][QN][4];
 #pragma unroll
-        for (int c = 0; c < SK / 16; ++c) {
-            const int pc = (c * 16) / p.piece, in = c * 16 - pc * p.piece;
+        for (int c = 0; c < NC; ++c) {
+            const int pc = FAST ? 0 : (c * 16) >> piece_log, in = c * 16 - pc * piece;
             const uint8_t* base = ks + pc * piece_bytes;
-            const uint8_t* par = base + p.piece * (p.head_dim / 2) + in * NG * 4;
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                float (&sc)[2 * RH] = s[2 * c + t];
-#pragma unroll
-                for (int e = 0; e < 2 * RH; ++e) sc[e] = 0.0f;
-                uint32_t pr[2][NG];
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    pr[0][g] = *reinterpret_cast<const uint32_t*>(par + ((t * 8 + 2 * j) * NG + g) * 4);
-                    pr[1][g] = *reinterpret_cast<const uint32_t*>(par + ((t * 8 + 2 * j + 1) * NG + g) * 4);
-                }
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const bool sh = g == NG - 1 && short_last;
-                    const int off = sh ? (in + t * 8 + n) * 8 + (j & 1) * 4 : (in + t * 8 + n) * 16 + j * 4;
-                    const uint32_t w = *reinterpret_cast<const uint32_t*>(base + g * p.piece * 16 + off);
-                    const uint32_t b0 = code_pair(w, 0), b1 = code_pair(w, 1), b2 = code_pair(w, 2), b3 = code_pair(w, 3);
-                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int z = PIECES - 1; z >= 0; --z) {
-                        if (LOW) {
-                            mma(acc, qa[g][0][z][0], 0u, qa[g][0][z][RH], 0u, b0, b1);
-                            mma(acc, qa[g][1][z][0], 0u, qa[g][1][z][RH], 0u, b2, b3);
-                        } else {
-                            mma(acc, qa[g][0][z][0], qa[g][0][z][1 % (2 * RH)], qa[g][0][z][RH], qa[g][0][z][(RH + 1) % (2 * RH)], b0, b1);
-                            mma(acc, qa[g][1][z][0], qa[g][1][z][1 % (2 * RH)], qa[g][1][z][RH], qa[g][1][z][(RH + 1) % (2 * RH)], b2, b3);
-                        }
-                    }
-#pragma unroll
-                    for (int r = 0; r < RH; ++r)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float step = __uint_as_float(pr[e][g] << 16);
-                            const float middle = __uint_as_float(pr[e][g] & 0xffff0000u);
-                            sc[2 * r + e] = fmaf(step, acc[2 * r + e], fmaf(middle, qsum[g][r], sc[2 * r + e]));
-                        }
-                }
-            }
-        }
-        // ---- mask, maximum, exponentials
-        float alpha[RH];
-#pragma unroll
-        for (int r = 0; r < RH; ++r) {
-            const int row = n + 8 * r;
-            const int pos = pos0 + (first + min(row, rows - 1)) / p.hpg;
-            float top = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float v = s[t][2 * r + e] * sl2;
-                    if (masked) {
-                        const int key = key0 + t * 8 + 2 * j + e;
-                        if (key > pos || (p.window > 0 && key <= pos - p.window)) v = -INFINITY;
-                    }
-                    s[t][2 * r + e] = v;
-                    top = fmaxf(top, v);
-                }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float now = fmaxf(m[r], top);
-            const float ref = now == -INFINITY ? 0.0f : now;
-            alpha[r] = exp2_fast(m[r] - ref);                 // (0 while nothing was seen)
-            m[r] = now;
-            float sum = 0.0f;
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    s[t][2 * r + e] = exp2_fast(s[t][2 * r + e] - ref);
-                    sum += s[t][2 * r + e];
-                }
-            l[r] = l[r] * alpha[r] + sum;
-        }
-        bool moved = alpha[0] != 1.0f;
-        if (RH == 2) moved = moved || alpha[RH - 1] != 1.0f;
-        if (__any_sync(0xffffffffu, moved)) {
+            const uint8_t* par = base + piece * (head_dim / 2) + (in + n) * NG * 4;
+            uint32_t pr[2][NG];
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-#pragma unroll
-                for (int r = 0; r < RH; ++r) mid[g][r] *= alpha[r];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int r = 0; r < RH; ++r) {
-                        o[g][i][2 * r] *= alpha[r];
-                        o[g][i][2 * r + 1] *= alpha[r];
-                    }
+                pr[0][g] = *reinterpret_cast<const uint32_t*>(par + g * 4);
+                pr[1][g] = *reinterpret_cast<const uint32_t*>(par + 8 * NG * 4 + g * 4);
             }
+#pragma unroll
+            for (int z = 0; z < QN; ++z)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[c][z][e] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const bool sh = g == NG - 1 && short_last;
+                const uint8_t* word = base + g * piece * 16 + (sh ? (in + n) * 8 + (j & 1) * 4 : (in + n) * 16 + j * 4);
+                const uint32_t w0 = *reinterpret_cast<const uint32_t*>(word);
+                const uint32_t w1 = *reinterpret_cast<const uint32_t*>(word + (sh ? 64 : 128));
+                float step[2], rest[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    step[e] = __uint_as_float(pr[e][g] << 16);
+                    rest[e] = __uint_as_float(pr[e][g] & 0xffff0000u);
+                    if (!EXACT) rest[e] = fmaf(step[e], -136.0f, rest[e]);
+                }
+                uint32_t a[4][2];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    a[i][0] = code_pair<EXACT>(w0, i);
+                    a[i][1] = code_pair<EXACT>(w1, i);
+                }
+#pragma unroll
+                for (int z = 0; z < QN; ++z) {
+                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int y = PIECES - 1; y >= 0; --y) {
+                        mma(acc, a[0][0], a[0][1], a[1][0], a[1][1], qb[z][g][0][y][0], qb[z][g][0][y][1]);
+                        mma(acc, a[2][0], a[2][1], a[3][0], a[3][1], qb[z][g][1][y][0], qb[z][g][1][y][1]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[c][z][e] = fmaf(step[e >> 1], acc[e], fmaf(rest[e >> 1], qsum[z][g][e & 1], s[c][z][e]));
+                }
+            }
+        }
+        if (masked) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int z = 0; z < QN; ++z)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = key0 + c * 16 + n + 8 * (e >> 1);
+                        if (key > pos[z][e & 1] || (p.window > 0 && key <= pos[z][e & 1] - p.window)) s[c][z][e] = -INFINITY;
+                    }
+        }
+        // ---- maximum, exponentials
+        float alpha[QN][2];
+        bool moved = false;
+#pragma unroll
+        for (int z = 0; z < QN; ++z)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) top = fmaxf(top, fmaxf(s[c][z][e], s[c][z][e + 2]));
+#pragma unroll
+                for (int o2 = 4; o2 < 32; o2 <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o2));
+                const float now = fmaxf(m[z][e], top * sl2);
+                const float ref = now == -INFINITY ? 0.0f : now;
+                alpha[z][e] = exp2_fast(m[z][e] - ref);       // (0 while nothing was seen)
+                moved = moved || alpha[z][e] != 1.0f;
+                m[z][e] = now;
+                float sum = 0.0f;
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int k = e; k < 4; k += 2) {
+                        s[c][z][k] = exp2_fast(fmaf(s[c][z][k], sl2, -ref));
+                        sum += s[c][z][k];
+                    }
+                l[z][e] = fmaf(l[z][e], alpha[z][e], sum);
+            }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int z = 0; z < QN; ++z)
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        mid[z][g][e] *= alpha[z][e];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            o[z][g][i][e] *= alpha[z][e];
+                            o[z][g][i][e + 2] *= alpha[z][e];
+                        }
+                    }
         }
         // ---- values
 #pragma unroll
-        for (int c = 0; c < SK / 16; ++c) {
-            const int pc = (c * 16) / p.piece, in = c * 16 - pc * p.piece;
+        for (int c = 0; c < NC; ++c) {
+            const int pc = FAST ? 0 : (c * 16) >> piece_log, in = c * 16 - pc * piece;
             const uint8_t* base = vs + pc * piece_bytes;
-            const uint8_t* par = base + p.piece * (p.head_dim / 2) + in * NG * 4;
+            const uint8_t* par = base + piece * (head_dim / 2) + (in + n) * NG * 4;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                // p * step of keys 2 j, 2 j + 1 (tile 0) and 8 + 2 j, 9 + 2 j (tile 1)
-                uint32_t a[PIECES][2][RH];
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const uint32_t p0 = *reinterpret_cast<const uint32_t*>(par + ((t * 8 + 2 * j) * NG + g) * 4);
-                    const uint32_t p1 = *reinterpret_cast<const uint32_t*>(par + ((t * 8 + 2 * j + 1) * NG + g) * 4);
-#pragma unroll
-                    for (int r = 0; r < RH; ++r) {
-                        const float w0 = s[2 * c + t][2 * r], w1 = s[2 * c + t][2 * r + 1];
-                        float x0 = w0 * __uint_as_float(p0 << 16), x1 = w1 * __uint_as_float(p1 << 16);
-                        float y0 = w0 * __uint_as_float(p0 & 0xffff0000u), y1 = w1 * __uint_as_float(p1 & 0xffff0000u);
-                        if (masked) {
-                            // (a masked key's step and middle may be anything, NaN too)
-                            if (w0 == 0.0f) x0 = y0 = 0.0f;
-                            if (w1 == 0.0f) x1 = y1 = 0.0f;
-                        }
-                        mid[g][r] += y0 + y1;
-                        uint32_t w[PIECES];
-                        split2<PIECES>(x0, x1, w);
-#pragma unroll
-                        for (int z = 0; z < PIECES; ++z) a[z][t][r] = w[z];
-                    }
-                }
                 const bool sh = g == NG - 1 && short_last;
-                const uint8_t* col = base + g * p.piece * 16 + (sh ? (n & 1) * 4 : (n & 3) * 4) + (n >> 2) * 2;
-                const int row = sh ? 8 : 16;
-                auto half = [&](int key) -> uint32_t { return *reinterpret_cast<const uint16_t*>(col + (in + key) * row); };
+                const uint8_t* col = base + g * piece * 16 + (sh ? (n & 1) * 4 : (n & 3) * 4) + (n >> 2) * 2;
+                auto half = [&](int key) -> uint32_t {
+                    return *reinterpret_cast<const uint16_t*>(col + (in + key) * (sh ? 8 : 16));
+                };
                 const uint32_t u = half(2 * j) | (half(2 * j + 1) << 16);
                 const uint32_t v = half(8 + 2 * j) | (half(9 + 2 * j) << 16);
+                uint32_t a[4][2];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t b0 = code_pair(u, i), b1 = code_pair(v, i);
+                    a[i][0] = code_pair<true>(u, i);
+                    a[i][1] = code_pair<true>(v, i);
+                }
+                float step[2], middle[2];
 #pragma unroll
-                    for (int z = PIECES - 1; z >= 0; --z) {
-                        if (LOW)
-                            mma(o[g][i], a[z][0][0], 0u, a[z][1][0], 0u, b0, b1);
-                        else
-                            mma(o[g][i], a[z][0][0], a[z][0][RH - 1], a[z][1][0], a[z][1][RH - 1], b0, b1);
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t pr = *reinterpret_cast<const uint32_t*>(par + e * 8 * NG * 4 + g * 4);
+                    step[e] = __uint_as_float(pr << 16);
+                    middle[e] = __uint_as_float(pr & 0xffff0000u);
+                }
+#pragma unroll
+                for (int z = 0; z < QN; ++z) {
+                    float x[4], y[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x[e] = s[c][z][e] * step[e >> 1];
+                        y[e] = s[c][z][e] * middle[e >> 1];
+                    }
+                    if (masked) {
+                        // (a masked key's step and middle may be anything, NaN too)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (s[c][z][e] == 0.0f) x[e] = y[e] = 0.0f;
+                    }
+                    mid[z][g][0] += y[0] + y[2];
+                    mid[z][g][1] += y[1] + y[3];
+                    uint32_t b0[PIECES], b1[PIECES];
+                    split2<PIECES>(x[0], x[1], b0);
+                    split2<PIECES>(x[2], x[3], b1);
+#pragma unroll
+                    for (int k = PIECES - 1; k >= 0; --k) {
+                        const uint32_t t0 = transpose8(b0[k]), t1 = transpose8(b1[k]);
+                        mma(o[z][g][0], a[0][0], a[1][0], a[0][1], a[1][1], t0, t1);
+                        mma(o[z][g][1], a[2][0], a[3][0], a[2][1], a[3][1], t0, t1);
                     }
                 }
             }
         }
         __syncwarp();                                          // every lane has read the stage
-        if (blk + STAGES * WARPS < my_hi) {
-            request(blk + STAGES * WARPS, st, ahead);
-            ahead = page_of(blk + (STAGES + 1) * WARPS);
+        if (blk + STAGES * p.warps < my_hi) {
+            request(blk + STAGES * p.warps, st, ahead);
+            ahead = page_of(blk + (STAGES + 1) * p.warps);
         }
     }
     if (!alive) {
         // wait (bounded) for the copies still on their way before the ring takes the states
         for (int s2 = 0; s2 < STAGES; ++s2) {
-            const int i2 = it + s2, blk = my_lo + warp + i2 * WARPS;
+            const int i2 = it + s2, blk = my_lo + warp + i2 * p.warps;
             if (blk >= my_hi) break;
             for (uint32_t i = 0; i < WAIT_LIMIT; ++i)
                 if (mbar_try_wait(bar0 + (i2 % STAGES) * 8, (i2 / STAGES) & 1)) break;
@@ -468,69 +503,68 @@ __global__ void __launch_bounds__(THREADS) attention_4bit_kernel(const Args p) {
     __syncwarp();
 
     // ------------------------------------------------- the warps' states, then the cluster's
-    float* mine = reinterpret_cast<float*>(smem + warp * STAGES * L::STAGE);
+    float* mine = reinterpret_cast<float*>(smem + warp * L::WARP);
 #pragma unroll
-    for (int r = 0; r < RH; ++r) {
-        float sum = l[r];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        float* st = mine + (n + 8 * r) * PART;
-        if (j == 0) {
-            st[DP] = m[r];
+    for (int z = 0; z < QN; ++z)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float sum = l[z][e];
+#pragma unroll
+            for (int o2 = 4; o2 < 32; o2 <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o2);
+            const int row = 8 * z + 2 * j + e;
+            float* st = mine + row * PART;
+            if (n == 0) {
+                st[DP] = m[z][e];
+                st[DP + 1] = sum;
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                float y = mid[z][g][e];
+#pragma unroll
+                for (int o2 = 4; o2 < 32; o2 <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o2);
+                float* at = st + g * 32 + 8 * (n & 3) + 4 * (n >> 2);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    at[2 * i] = o[z][g][i][e] + y;
+                    at[2 * i + 1] = o[z][g][i][e + 2] + y;
+                }
+            }
+        }
+    __syncthreads();
+    if (p.warps > 1) {
+        // (a thread owns its column of every warp's state; the maxima and sums are left alone until all have read them)
+        for (int e = threadIdx.x; e < rows * DP; e += threads) {
+            const int row = e / DP, ch = e - row * DP;
+            float top = -INFINITY, x = 0.0f;
+            for (int w = 0; w < p.warps; ++w)
+                top = fmaxf(top, reinterpret_cast<const float*>(smem + w * L::WARP)[row * PART + DP]);
+            for (int w = 0; w < p.warps; ++w) {
+                const float* st = reinterpret_cast<const float*>(smem + w * L::WARP) + row * PART;
+                x += (st[DP] == -INFINITY ? 0.0f : exp2_fast(st[DP] - top)) * st[ch];
+            }
+            reinterpret_cast<float*>(smem)[row * PART + ch] = x;
+        }
+        __syncthreads();
+        if (threadIdx.x < rows) {
+            const int row = threadIdx.x;
+            float top = -INFINITY, sum = 0.0f;
+            for (int w = 0; w < p.warps; ++w)
+                top = fmaxf(top, reinterpret_cast<const float*>(smem + w * L::WARP)[row * PART + DP]);
+            for (int w = 0; w < p.warps; ++w) {
+                const float* st = reinterpret_cast<const float*>(smem + w * L::WARP) + row * PART;
+                sum += (st[DP] == -INFINITY ? 0.0f : exp2_fast(st[DP] - top)) * st[DP + 1];
+            }
+            float* st = reinterpret_cast<float*>(smem) + row * PART;
+            st[DP] = top;
             st[DP + 1] = sum;
         }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            float y = mid[g][r];
-            y += __shfl_xor_sync(0xffffffffu, y, 1);
-            y += __shfl_xor_sync(0xffffffffu, y, 2);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int col = 2 * j + e;
-                    st[g * 32 + 8 * (col & 3) + 4 * (col >> 2) + i] = o[g][i][2 * r + e] + y;
-                }
-        }
-    }
-    __syncthreads();
-    // (column by column: a thread owns its columns of every warp's state, the rows' maxima and sums are left alone)
-    for (int e = threadIdx.x; e < rows * DP; e += THREADS) {
-        const int row = e / DP, ch = e - row * DP;
-        float top = -INFINITY, x = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w)
-            top = fmaxf(top, reinterpret_cast<const float*>(smem + w * STAGES * L::STAGE)[row * PART + DP]);
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const float* st = reinterpret_cast<const float*>(smem + w * STAGES * L::STAGE) + row * PART;
-            const float f = st[DP] == -INFINITY ? 0.0f : exp2_fast(st[DP] - top);
-            x += f * st[ch];
-        }
-        reinterpret_cast<float*>(smem)[row * PART + ch] = x;
-    }
-    __syncthreads();
-    if (threadIdx.x < rows) {
-        const int row = threadIdx.x;
-        float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w)
-            top = fmaxf(top, reinterpret_cast<const float*>(smem + w * STAGES * L::STAGE)[row * PART + DP]);
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const float* st = reinterpret_cast<const float*>(smem + w * STAGES * L::STAGE) + row * PART;
-            sum += (st[DP] == -INFINITY ? 0.0f : exp2_fast(st[DP] - top)) * st[DP + 1];
-        }
-        float* st = reinterpret_cast<float*>(smem) + row * PART;
-        st[DP] = top;
-        st[DP + 1] = sum;
     }
     if (p.parts > 1)
         cluster_sync_all();
     else
         __syncthreads();
     const uint32_t state = smem_u32(smem);
-    for (int e = rank * THREADS + threadIdx.x; e < rows * DP; e += THREADS * p.parts) {
+    for (int e = rank * threads + threadIdx.x; e < rows * DP; e += threads * p.parts) {
         const int row = e / DP, ch = e - row * DP;
         float x, sum;
         if (p.parts == 1) {
@@ -549,24 +583,23 @@ __global__ void __launch_bounds__(THREADS) attention_4bit_kernel(const Args p) {
                 sum += f * lds_cluster(at + (DP + 1) * 4);
             }
         }
-        if (ch < p.head_dim) {
+        if (ch < head_dim) {
             const int at = first + row, tk = at / p.hpg, h = hk * p.hpg + at - tk * p.hpg;
-            reinterpret_cast<T*>(p.out)[(long)(row0 + tk) * p.out_stride + (long)h * p.head_dim + ch] =
+            reinterpret_cast<T*>(p.out)[(long)(row0 + tk) * p.out_stride + (long)h * head_dim + ch] =
                 prb_from_float<T>(sum > 0.0f ? x / sum : 0.0f);
         }
     }
     if (p.parts > 1) cluster_sync_all();                       // nobody leaves while its state may be read
 }
 
-template <int NG, bool LOW, typename T> int launch_one(const Args& p, cudaStream_t stream) {
-    using L = Layout<NG>;
-    constexpr int bytes = L::RING + L::BARS + 16;
-    cudaError_t e = prb_allow_shared<attention_4bit_kernel<NG, LOW, T>>(bytes);
+template <int NG, int QN, typename T, bool FAST> int launch_one(const Args& p, cudaStream_t stream) {
+    using L = Layout<NG, QN>;
+    cudaError_t e = prb_allow_shared<attention_4bit_kernel<NG, QN, T, FAST>>(L::bytes(MAX_WARPS));
     if (e != cudaSuccess) return (int)e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((long)p.n_tiles * p.kv_heads * p.subs * p.parts));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = bytes;
+    cfg.blockDim = dim3(p.warps * 32);
+    cfg.dynamicSmemBytes = L::bytes(p.warps);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -577,7 +610,26 @@ template <int NG, bool LOW, typename T> int launch_one(const Args& p, cudaStream
     attr[1].val.programmaticStreamSerializationAllowed = prb_small_ctas_early() && prb_pdl_enabled() ? 1 : 0;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, attention_4bit_kernel<NG, LOW, T>, p);
+    e = cudaLaunchKernelEx(&cfg, attention_4bit_kernel<NG, QN, T, FAST>, p);
     return e == cudaSuccess ? 0 : (int)e;
+}
+
+// `p` but for subs, parts, warps and piece is set; rows: the most rows of a tile.
+template <int NG, int QN, typename T> int launch_by(Args p, long rows, int max_context, int parts, cudaStream_t stream) {
+    constexpr int sk = stage_keys(NG, QN);
+    p.piece = p.page_size % sk == 0 ? sk : p.page_size % 32 == 0 ? 32 : 16;
+    if (sk % p.page_size == 0) p.piece = p.page_size;
+    const long subs = (rows + 8 * QN - 1) / (8 * QN), units = (long)p.n_tiles * p.kv_heads * subs;
+    if (units > 0x7fffffffL / MAX_PARTS) return PRB_E_SIZE;
+    p.subs = (int)subs;
+    p.warps = MAX_WARPS;
+    // Parts of a unit's keys: as many as give every SM about four CTAs, each with a stage a warp at least.
+    const int span = p.window > 0 && p.window < max_context ? p.window + sk : max_context;
+    const int stages = (span + sk - 1) / sk;
+    p.parts = 1;
+    while (p.parts < MAX_PARTS && units * p.parts * 2 <= 4L * prb_sm_count() && stages >= p.parts * 2 * p.warps) p.parts *= 2;
+    if (parts > 0) p.parts = parts;
+    if (p.piece == sk && p.head_dim == 32 * NG) return launch_one<NG, QN, T, true>(p, stream);
+    return launch_one<NG, QN, T, false>(p, stream);
 }
 }  // namespace attn4
