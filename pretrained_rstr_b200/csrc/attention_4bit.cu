@@ -6,13 +6,17 @@ int prb_attention_4bit_f32(const attn4::Args& p, long rows, int max_context, int
 int prb_attention_4bit_rows(const attn4::Args& p, long rows, int max_context, int parts, cudaStream_t stream);
 
 namespace {
-// up to 8 rows a tile
+// up to 4 rows a tile, or 8
+template <int NG> int by(const attn4::Args& p, long rows, int max_context, int parts, cudaStream_t stream) {
+    return rows <= 4 ? attn4::launch_by<NG, 1, 1, __nv_bfloat16>(p, rows, max_context, parts, stream)
+                     : attn4::launch_by<NG, 1, 2, __nv_bfloat16>(p, rows, max_context, parts, stream);
+}
 int launch_few(const attn4::Args& p, long rows, int max_context, int parts, cudaStream_t stream) {
     switch (cache4::groups_of(p.head_dim)) {
-        case 1: return attn4::launch_by<1, 1, __nv_bfloat16>(p, rows, max_context, parts, stream);
-        case 2: return attn4::launch_by<2, 1, __nv_bfloat16>(p, rows, max_context, parts, stream);
-        case 3: return attn4::launch_by<3, 1, __nv_bfloat16>(p, rows, max_context, parts, stream);
-        default: return attn4::launch_by<4, 1, __nv_bfloat16>(p, rows, max_context, parts, stream);
+        case 1: return by<1>(p, rows, max_context, parts, stream);
+        case 2: return by<2>(p, rows, max_context, parts, stream);
+        case 3: return by<3>(p, rows, max_context, parts, stream);
+        default: return by<4>(p, rows, max_context, parts, stream);
     }
 }
 }  // namespace
@@ -45,6 +49,7 @@ PRB_API int prb_attention_4bit(void* out, long out_stride, const void* q, long q
     p.scale = scale; p.window = window;
     p.wide = (uintptr_t)q % 16 == 0 && (q_stride * size) % 16 == 0;
     p.status = status;
+    p.magic = 0x43004300u;
     const long rows = (long)tile_most * hpg;
     if (dtype == PRB_F32) return prb_attention_4bit_f32(p, rows, max_context, parts, stream);
     return rows <= 8 ? launch_few(p, rows, max_context, parts, stream)

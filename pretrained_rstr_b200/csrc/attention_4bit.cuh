@@ -14,8 +14,8 @@
 // Keys and values are the left operand (16 keys x 16 channels, 16 channels x 16 keys), queries and probabilities the
 // right one (8 rows a product): one decoded token with a key/value head of its own wastes 7 of 8 columns rather than
 // 15 of 16 rows, a thread looks after the steps and middles of 2 keys in 16 rather than 4, and half as many products do.  The
-// scores' accumulator has keys along lanes where the probabilities' operand has rows there: a transposing move of an
-// 8 x 8 block of the rounded numbers (movmatrix) turns one into the other.
+// scores' accumulator has keys along lanes where the probabilities' operand has rows there: the rounded numbers change
+// lanes by shuffles (as_operand).
 //
 // What bounds it: the instructions that turn words of codes into operands and scale them; then the bytes of the cache.
 // With bfloat16 queries the 8 stays in the codes of the keys (128 + c is what the bits of a code make without an
@@ -27,6 +27,8 @@
 // Each of its warps takes every nth stage of SK keys and keeps two stages of its own in flight (bulk copies, no
 // multicast, of whole tiles where a page is a stage).  Nothing is shared between warps until the end.
 #pragma once
+#include <type_traits>
+
 #include "cache4.cuh"
 #include "tcgen05.cuh"
 
@@ -62,6 +64,7 @@ struct Args {
     int tile_bytes;
     float scale;
     int window;
+    uint32_t magic;                        // 0x43004300 (see code_pair)
     int wide;                              // queries can be read 16 bytes at a time
     int* status;
 };
@@ -78,19 +81,34 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same from nothing: d = a b.
+__device__ __forceinline__ void mma0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                     uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// 16 x 8 x 8
+__device__ __forceinline__ void mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(b0));
+}
+__device__ __forceinline__ void mma8_0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(b0), "f"(0.0f));
+}
 // Codes i and i + 4 of a word as two bfloat16 numbers: 0x4300 | c is 128 + c; less 136 if CENTRED.
-template <bool CENTRED> __device__ __forceinline__ uint32_t code_pair(uint32_t word, int i) {
-    const uint32_t u = ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+// `magic` comes from the launch: of two constants the compiler keeps neither in a register and spends an instruction more
+// on every pair, an eighth of the kernel's.
+template <bool CENTRED> __device__ __forceinline__ uint32_t code_pair(uint32_t word, int i, uint32_t magic) {
+    const uint32_t u = ((word >> (4 * i)) & 0x000f000fu) | magic;
     if (!CENTRED) return u;
     const __nv_bfloat162 off = __floats2bfloat162_rn(136.0f, 136.0f);
     const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), off);
     return *reinterpret_cast<const uint32_t*>(&v);
-}
-// Row r, columns 2 c and 2 c + 1 of an 8 x 8 block in lane 4 r + c -> the same of its transpose.
-__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
-    uint32_t y;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -123,8 +141,48 @@ template <int PIECES> __device__ __forceinline__ void split2(float x, float y, u
     }
 }
 
-template <int NG, int QN> struct Layout {
-    static constexpr int SK = stage_keys(NG, QN), ROWS = 8 * QN;
+// Rows' numbers of keys n and n + 8 (lane 4 n + j: rows 2 j and 2 j + 1, or row j where EN is 1), rounded, as the right
+// operand of a product over 16 keys: columns are rows, and its reduction's places 2 j, 2 j + 1 are keys j, j + 8, its
+// places 2 j + 8, 2 j + 9 keys j + 4, j + 12, so that one pair moves at a time and nothing is put together again.
+// (movmatrix would do it in the keys' own order, but is made of a dozen instructions here.)
+template <int EN, int PIECES>
+__device__ __forceinline__ void as_operand(const float (&x)[2 * EN], int lane, uint32_t (&b0)[PIECES], uint32_t (&b1)[PIECES]) {
+    const int from = (lane & 3) * 4 + (lane >> 3);
+    uint32_t even[PIECES];
+    split2<PIECES>(x[0], x[EN], even);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        b0[i] = __shfl_sync(0xffffffffu, even[i], from);
+        b1[i] = __shfl_sync(0xffffffffu, even[i], from + 16);
+    }
+    if (EN == 2) {
+        uint32_t odd[PIECES];
+        split2<PIECES>(x[1 % (2 * EN)], x[3 % (2 * EN)], odd);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const uint32_t o0 = __shfl_sync(0xffffffffu, odd[i], from), o1 = __shfl_sync(0xffffffffu, odd[i], from + 16);
+            if (lane & 4) {
+                b0[i] = o0;
+                b1[i] = o1;
+            }
+        }
+    }
+}
+// The (step, middle) pairs of a key's groups.
+template <int NG> __device__ __forceinline__ void load_params(const uint8_t* p, uint32_t (&out)[NG]) {
+    if (NG == 4) {
+        const uint4 w = *reinterpret_cast<const uint4*>(p);
+        out[0] = w.x; out[1 % NG] = w.y; out[2 % NG] = w.z; out[3 % NG] = w.w;
+    } else if (NG == 2) {
+        const uint2 w = *reinterpret_cast<const uint2*>(p);
+        out[0] = w.x; out[1 % NG] = w.y;
+    } else {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) out[g] = reinterpret_cast<const uint32_t*>(p)[g];
+    }
+}
+template <int NG, int QN, int EN> struct Layout {
+    static constexpr int SK = stage_keys(NG, QN), ROWS = EN == 1 ? 4 : 8 * QN;
     static constexpr int DP = NG * 32, PART = DP + 2;         // floats a row of a partial state: values, maximum, sum
     static constexpr int KIND = SK * (16 * NG + 4 * NG);      // most bytes of a stage's keys (and of its values)
     static constexpr int STAGE = 2 * KIND;
@@ -134,10 +192,13 @@ template <int NG, int QN> struct Layout {
     static constexpr int bytes(int warps) { return warps * (WARP + STAGES * 8) + 16; }
 };
 
-// FAST: the head size is 32 NG and a stage lies in one page, so that every offset is known here.
-template <int NG, int QN, typename T, bool FAST>
-__global__ void __launch_bounds__(MAX_WARPS * 32, QN == 1 ? (NG <= 2 ? 4 : 3) : 2) attention_4bit_kernel(const Args p) {
-    using L = Layout<NG, QN>;
+// QN: products' columns of 8 rows.  EN == 1 (QN is 1): up to 4 rows, in the columns 0, 2, 4 and 6, so that a thread has one
+// row's scores rather than two.  FAST: the head size is 32 NG and a stage lies in one page, so that every offset is known
+// here.
+template <int NG, int QN, int EN, typename T, bool FAST>
+__global__ void __launch_bounds__(MAX_WARPS * 32, QN > 1 ? 2 : NG > 2 && sizeof(T) == 4 ? 3 : 4)
+attention_4bit_kernel(const Args p) {
+    using L = Layout<NG, QN, EN>;
     constexpr int SK = L::SK, ROWS = L::ROWS, NC = SK / 16, DP = L::DP, PART = L::PART;
     constexpr int PIECES = sizeof(T) == 4 ? 3 : 1;
     constexpr bool EXACT = PIECES == 3;                       // codes less 8 in the keys' products too
@@ -191,15 +252,39 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, QN == 1 ? (NG <= 2 ? 4 : 3) : 
     const int piece_bytes = piece * (head_dim / 2 + 4 * NG);
     const int codes_of_page = p.page_size * (head_dim / 2);
     // Lane i looks after piece i of a stage: its page, ahead of time, and its copies.
+    const int per_page = FAST ? p.page_size / SK : 1;         // stages of a page
     auto page_of = [&](int blk) -> int {
+        if (FAST) return blk < my_hi ? table[per_page == 1 ? blk : blk / per_page] : -2;
         const int key = blk * SK + lane * piece;
         if (blk >= my_hi || lane >= pieces || key > pos_hi || key + piece <= key_lo) return -2;    // nothing to fetch
         return table[key / p.page_size];
     };
+    // (FAST: lane i has copy i of a stage, keys' and values' in turn: a page's tile, or its groups' codes and its pairs)
+    const int copy = lane >> 1;
+    const bool copies = FAST && copy < (per_page == 1 ? 1 : NG + 1);
+    const uint8_t* copy_from = (lane & 1 ? p.v_tiles : p.k_tiles) + (size_t)hk * p.tile_bytes +
+                               (copy < NG ? copy * p.page_size * 16 : codes_of_page);
+    const uint32_t copy_bytes = per_page == 1 ? L::KIND : SK * (copy < NG ? 16 : NG * 4);
+    const uint32_t copy_to = ring + (lane & 1) * L::KIND + copy * SK * 16;
+    const size_t page_stride = (size_t)p.kv_heads * p.tile_bytes;
     auto request = [&](int blk, int st, int page) {
+        if (FAST) {
+            const uint32_t bar = bar0 + st * 8;
+            const bool fine = page >= 0 && page < p.num_pages;
+            if (lane == 0) {
+                if (!fine) prb_set_status(p.status, PRB_S_PAGE_RANGE, row0, blk * SK, page);
+                mbar_expect_tx(bar, fine ? 2 * L::KIND : 0);
+            }
+            __syncwarp();
+            // (a page that is none: recorded, the stage keeps what it held, and the tile's result is not to be used)
+            if (copies && fine) {
+                const int at = per_page == 1 ? 0 : (blk % per_page) * SK * (copy < NG ? 16 : NG * 4);
+                bulk_load(copy_to + st * L::STAGE, copy_from + (size_t)page * page_stride + at, copy_bytes, bar);
+            }
+            return;
+        }
         bool fetch = page != -2;
         if (fetch && (page < 0 || page >= p.num_pages)) {
-            // (recorded; the stage keeps what it held, and the tile's result is not to be used)
             prb_set_status(p.status, PRB_S_PAGE_RANGE, row0, blk * SK + lane * piece, page);
             fetch = false;
         }
@@ -237,21 +322,26 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, QN == 1 ? (NG <= 2 ? 4 : 3) : 
     // Channel order of the reduction: thread j of a quad has channels 8 j + (i, i + 4), the codes that one shift and
     // one mask take from word j.
     uint32_t qb[QN][NG][2][PIECES][2];                        // [rows][group][half of the reduction][piece][operand]
-    float qsum[QN][NG][2];                                    // of rows 2 j and 2 j + 1
-    int pos[QN][2];
+    // What a key's steps and middles are multiplied by in a score, as three bfloat16 numbers each: less 136 sums of q
+    // (where the codes are 128 + c) and the sum of q, of group j.
+    uint32_t qp[QN][3];
+    int pos[QN][EN];
 #pragma unroll
     for (int z = 0; z < QN; ++z) {
-        const int row = n + 8 * z, at = first + min(row, rows - 1);
+        float mine = 0.0f;
+        // (column n of the products)
+        const int row = EN == 1 ? n >> 1 : n + 8 * z, at = first + min(row, rows - 1);
+        const bool used = row < rows && (EN == 2 || (n & 1) == 0);
         const int tk = at / p.hpg, h = hk * p.hpg + at - tk * p.hpg;
         const int here = pos0 + tk;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) pos[z][e] = __shfl_sync(0xffffffffu, here, (2 * j + e) * 4);
+        for (int e = 0; e < EN; ++e) pos[z][e] = __shfl_sync(0xffffffffu, here, (2 * j + e) * 4);
         const T* src = reinterpret_cast<const T*>(p.q) + (long)(row0 + tk) * p.q_stride + (long)h * head_dim;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             const int c0 = g * 32 + j * 8;
             float x[8];
-            if (row < rows && c0 < head_dim) {
+            if (used && c0 < head_dim) {
                 if (p.wide) {
                     if (sizeof(T) == 2) {
                         const uint4 w = *reinterpret_cast<const uint4*>(src + c0);
@@ -280,8 +370,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, QN == 1 ? (NG <= 2 ? 4 : 3) : 
             for (int i = 0; i < 8; ++i) sum += x[i];
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) qsum[z][g][e] = __shfl_sync(0xffffffffu, sum, (2 * j + e) * 4);
+            if (j == g) mine = sum;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 uint32_t w[PIECES];
@@ -290,91 +379,97 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, QN == 1 ? (NG <= 2 ? 4 : 3) : 
                 for (int y = 0; y < PIECES; ++y) qb[z][g][i >> 1][y][i & 1] = w[y];
             }
         }
+        split2<3>(EXACT ? 0.0f : -136.0f * mine, mine, qp[z]);
     }
 
-    // results [rows][group][16 of its channels]: channels (2 i, 2 i + 1 of the thread's four) x rows (2 j, 2 j + 1)
-    float o[QN][NG][2][4];
-    float mid[QN][NG][2], m[QN][2], l[QN][2];
+    // results [rows][group][16 of its channels]: channels (2 i, 2 i + 1 of the thread's four) x rows (2 j, 2 j + 1); sums of
+    // p * middle of group n
+    float o[QN][NG][2][4], mid[QN][4];
+    float m[QN][EN], l[QN][EN];
 #pragma unroll
-    for (int z = 0; z < QN; ++z)
+    for (int z = 0; z < QN; ++z) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        for (int e = 0; e < EN; ++e) {
             m[z][e] = -INFINITY;
             l[z][e] = 0.0f;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                mid[z][g][e] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[z][g][e][i] = 0.0f;
-            }
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            mid[z][i] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) o[z][g][0][i] = o[z][g][1][i] = 0.0f;
+        }
+    }
     const float sl2 = p.scale * 1.4426950408889634f;          // scores are handled in log2 units
     // (the short last group's rows are 8 bytes apart; its words 2 and 3 do not exist: words 0 and 1 stand in, against
     // queries of zero and for channels that are not stored)
     const bool short_last = !FAST && head_dim % 32 != 0;
 
-    bool alive = true;
-    int it = 0;
-    for (int blk = my_lo + warp; blk < my_hi; blk += p.warps, ++it) {
-        const int st = it % STAGES;
-        alive = mbar_wait_warp(bar0 + st * 8, (it / STAGES) & 1, failed);
-        if (!alive) {
-            if (lane == 0) prb_set_status(p.status, PRB_S_WAIT_TIMEOUT, 41, blockIdx.x, blk);
-            break;
-        }
+    const uint32_t magic = p.magic;
+    // A stage's keys and values: scores, exponentials, results.
+    auto work = [&](int st, int key0, auto masked_t) {
+        constexpr bool masked = decltype(masked_t)::value;
         const uint8_t* ks = ring_p + st * L::STAGE;
         const uint8_t* vs = ks + L::KIND;
-        const int key0 = blk * SK;
-        const bool masked = key0 + SK - 1 > pos_lo || (p.window > 0 && key0 <= pos_hi - p.window);
         // ---- scores of keys n and n + 8 of every 16
-        float s[NC][QN][4];
+        float s[NC][QN][2 * EN];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int pc = FAST ? 0 : (c * 16) >> piece_log, in = c * 16 - pc * piece;
             const uint8_t* base = ks + pc * piece_bytes;
             const uint8_t* par = base + piece * (head_dim / 2) + (in + n) * NG * 4;
             uint32_t pr[2][NG];
+            load_params<NG>(par, pr[0]);
+            load_params<NG>(par + 8 * NG * 4, pr[1]);
+            // steps and middles against the sums of q: numbers 2 j, 2 j + 1 of the reduction are group j's
+            const int jg = NG == 4 ? j : min(j, NG - 1);
+            const uint32_t p0 = *reinterpret_cast<const uint32_t*>(par + jg * 4);
+            const uint32_t p1 = *reinterpret_cast<const uint32_t*>(par + 8 * NG * 4 + jg * 4);
+            float sum[QN][4];
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                pr[0][g] = *reinterpret_cast<const uint32_t*>(par + g * 4);
-                pr[1][g] = *reinterpret_cast<const uint32_t*>(par + 8 * NG * 4 + g * 4);
+            for (int z = 0; z < QN; ++z) {
+                mma8_0(sum[z], p0, p1, qp[z][2]);
+                mma8(sum[z], p0, p1, qp[z][1]);
+                mma8(sum[z], p0, p1, qp[z][0]);
             }
-#pragma unroll
-            for (int z = 0; z < QN; ++z)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[c][z][e] = 0.0f;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 const bool sh = g == NG - 1 && short_last;
                 const uint8_t* word = base + g * piece * 16 + (sh ? (in + n) * 8 + (j & 1) * 4 : (in + n) * 16 + j * 4);
                 const uint32_t w0 = *reinterpret_cast<const uint32_t*>(word);
                 const uint32_t w1 = *reinterpret_cast<const uint32_t*>(word + (sh ? 64 : 128));
-                float step[2], rest[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    step[e] = __uint_as_float(pr[e][g] << 16);
-                    rest[e] = __uint_as_float(pr[e][g] & 0xffff0000u);
-                    if (!EXACT) rest[e] = fmaf(step[e], -136.0f, rest[e]);
-                }
                 uint32_t a[4][2];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    a[i][0] = code_pair<EXACT>(w0, i);
-                    a[i][1] = code_pair<EXACT>(w1, i);
+                    a[i][0] = code_pair<EXACT>(w0, i, magic);
+                    a[i][1] = code_pair<EXACT>(w1, i, magic);
                 }
+                const float step0 = __uint_as_float(pr[0][g] << 16), step1 = __uint_as_float(pr[1][g] << 16);
 #pragma unroll
                 for (int z = 0; z < QN; ++z) {
-                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float acc[4];
 #pragma unroll
                     for (int y = PIECES - 1; y >= 0; --y) {
-                        mma(acc, a[0][0], a[0][1], a[1][0], a[1][1], qb[z][g][0][y][0], qb[z][g][0][y][1]);
+                        if (y == PIECES - 1)
+                            mma0(acc, a[0][0], a[0][1], a[1][0], a[1][1], qb[z][g][0][y][0], qb[z][g][0][y][1]);
+                        else
+                            mma(acc, a[0][0], a[0][1], a[1][0], a[1][1], qb[z][g][0][y][0], qb[z][g][0][y][1]);
                         mma(acc, a[2][0], a[2][1], a[3][0], a[3][1], qb[z][g][1][y][0], qb[z][g][1][y][1]);
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[c][z][e] = fmaf(step[e >> 1], acc[e], fmaf(rest[e >> 1], qsum[z][g][e & 1], s[c][z][e]));
+                    for (int e = 0; e < EN; ++e) {
+                        sum[z][e] = fmaf(step0, acc[e], sum[z][e]);
+                        sum[z][e + 2] = fmaf(step1, acc[e + 2], sum[z][e + 2]);
+                    }
                 }
             }
+#pragma unroll
+            for (int z = 0; z < QN; ++z)
+#pragma unroll
+                for (int e = 0; e < EN; ++e) {
+                    s[c][z][e] = sum[z][e];
+                    s[c][z][e + EN] = sum[z][e + 2];
+                }
         }
         if (masked) {
 #pragma unroll
@@ -382,21 +477,21 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, QN == 1 ? (NG <= 2 ? 4 : 3) : 
 #pragma unroll
                 for (int z = 0; z < QN; ++z)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = key0 + c * 16 + n + 8 * (e >> 1);
-                        if (key > pos[z][e & 1] || (p.window > 0 && key <= pos[z][e & 1] - p.window)) s[c][z][e] = -INFINITY;
+                    for (int e = 0; e < 2 * EN; ++e) {
+                        const int key = key0 + c * 16 + n + 8 * (e / EN), at = pos[z][e % EN];
+                        if (key > at || (p.window > 0 && key <= at - p.window)) s[c][z][e] = -INFINITY;
                     }
         }
         // ---- maximum, exponentials
-        float alpha[QN][2];
+        float alpha[QN][EN];
         bool moved = false;
 #pragma unroll
         for (int z = 0; z < QN; ++z)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
+            for (int e = 0; e < EN; ++e) {
                 float top = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < NC; ++c) top = fmaxf(top, fmaxf(s[c][z][e], s[c][z][e + 2]));
+                for (int c = 0; c < NC; ++c) top = fmaxf(top, fmaxf(s[c][z][e], s[c][z][e + EN]));
 #pragma unroll
                 for (int o2 = 4; o2 < 32; o2 <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o2));
                 const float now = fmaxf(m[z][e], top * sl2);
@@ -408,7 +503,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, QN == 1 ? (NG <= 2 ? 4 : 3) : 
 #pragma unroll
                 for (int c = 0; c < NC; ++c)
 #pragma unroll
-                    for (int k = e; k < 4; k += 2) {
+                    for (int k = e; k < 2 * EN; k += EN) {
                         s[c][z][k] = exp2_fast(fmaf(s[c][z][k], sl2, -ref));
                         sum += s[c][z][k];
                     }
@@ -418,23 +513,55 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, QN == 1 ? (NG <= 2 ? 4 : 3) : 
 #pragma unroll
             for (int z = 0; z < QN; ++z)
 #pragma unroll
-                for (int g = 0; g < NG; ++g)
+                for (int i = 0; i < 4; ++i) {
+                    if ((i & 1) >= EN) continue;
+                    const float by = alpha[z][(i & 1) % EN];
+                    mid[z][i] *= by;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        mid[z][g][e] *= alpha[z][e];
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            o[z][g][i][e] *= alpha[z][e];
-                            o[z][g][i][e + 2] *= alpha[z][e];
-                        }
+                    for (int g = 0; g < NG; ++g) {
+                        o[z][g][0][i] *= by;
+                        o[z][g][1][i] *= by;
                     }
+                }
         }
         // ---- values
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int pc = FAST ? 0 : (c * 16) >> piece_log, in = c * 16 - pc * piece;
             const uint8_t* base = vs + pc * piece_bytes;
-            const uint8_t* par = base + piece * (head_dim / 2) + (in + n) * NG * 4;
+            const uint8_t* par = base + piece * (head_dim / 2) + in * NG * 4;
+            uint32_t pr[2][NG];
+            load_params<NG>(par + n * NG * 4, pr[0]);
+            load_params<NG>(par + (n + 8) * NG * 4, pr[1]);
+            if (!masked) {
+                // p * middle: rows of the left operand are groups (n, those beyond the last stand in for themselves)
+                const uint8_t* col = par + (NG == 1 ? 0 : NG == 2 ? (n & 1) : NG == 4 ? (n & 3) : min(n, 2)) * 4 + 2;
+                auto middle = [&](int key) -> uint32_t { return *reinterpret_cast<const uint16_t*>(col + key * NG * 4); };
+                const uint32_t a0 = middle(j) | (middle(j + 8) << 16);
+                const uint32_t a1 = middle(j + 4) | (middle(j + 12) << 16);
+#pragma unroll
+                for (int z = 0; z < QN; ++z) {
+                    uint32_t b0[PIECES], b1[PIECES];
+                    as_operand<EN, PIECES>(s[c][z], lane, b0, b1);
+#pragma unroll
+                    for (int k = PIECES - 1; k >= 0; --k) mma(mid[z], a0, 0u, a1, 0u, b0[k], b1[k]);
+                }
+            } else {
+                // A masked key's middle may be anything, NaN too, which a product would spread over all rows.
+#pragma unroll
+                for (int z = 0; z < QN; ++z)
+#pragma unroll
+                    for (int e = 0; e < EN; ++e)
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) {
+                            float y = 0.0f;
+                            if (s[c][z][e] != 0.0f) y += s[c][z][e] * __uint_as_float(pr[0][g] & 0xffff0000u);
+                            if (s[c][z][e + EN] != 0.0f) y += s[c][z][e + EN] * __uint_as_float(pr[1][g] & 0xffff0000u);
+#pragma unroll
+                            for (int o2 = 4; o2 < 32; o2 <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o2);
+                            if (n == g) mid[z][e] += y;
+                        }
+            }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 const bool sh = g == NG - 1 && short_last;
@@ -442,49 +569,54 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, QN == 1 ? (NG <= 2 ? 4 : 3) : 
                 auto half = [&](int key) -> uint32_t {
                     return *reinterpret_cast<const uint16_t*>(col + (in + key) * (sh ? 8 : 16));
                 };
-                const uint32_t u = half(2 * j) | (half(2 * j + 1) << 16);
-                const uint32_t v = half(8 + 2 * j) | (half(9 + 2 * j) << 16);
+                const uint32_t u = half(j) | (half(j + 8) << 16);
+                const uint32_t v = half(j + 4) | (half(j + 12) << 16);
                 uint32_t a[4][2];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    a[i][0] = code_pair<true>(u, i);
-                    a[i][1] = code_pair<true>(v, i);
+                    a[i][0] = code_pair<true>(u, i, magic);
+                    a[i][1] = code_pair<true>(v, i, magic);
                 }
-                float step[2], middle[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t pr = *reinterpret_cast<const uint32_t*>(par + e * 8 * NG * 4 + g * 4);
-                    step[e] = __uint_as_float(pr << 16);
-                    middle[e] = __uint_as_float(pr & 0xffff0000u);
-                }
+                const float step0 = __uint_as_float(pr[0][g] << 16), step1 = __uint_as_float(pr[1][g] << 16);
 #pragma unroll
                 for (int z = 0; z < QN; ++z) {
-                    float x[4], y[4];
+                    float x[2 * EN];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[e] = s[c][z][e] * step[e >> 1];
-                        y[e] = s[c][z][e] * middle[e >> 1];
+                    for (int e = 0; e < EN; ++e) {
+                        x[e] = s[c][z][e] * step0;
+                        x[e + EN] = s[c][z][e + EN] * step1;
+                        if (masked) {
+                            if (s[c][z][e] == 0.0f) x[e] = 0.0f;
+                            if (s[c][z][e + EN] == 0.0f) x[e + EN] = 0.0f;
+                        }
                     }
-                    if (masked) {
-                        // (a masked key's step and middle may be anything, NaN too)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (s[c][z][e] == 0.0f) x[e] = y[e] = 0.0f;
-                    }
-                    mid[z][g][0] += y[0] + y[2];
-                    mid[z][g][1] += y[1] + y[3];
                     uint32_t b0[PIECES], b1[PIECES];
-                    split2<PIECES>(x[0], x[1], b0);
-                    split2<PIECES>(x[2], x[3], b1);
+                    as_operand<EN, PIECES>(x, lane, b0, b1);
 #pragma unroll
                     for (int k = PIECES - 1; k >= 0; --k) {
-                        const uint32_t t0 = transpose8(b0[k]), t1 = transpose8(b1[k]);
-                        mma(o[z][g][0], a[0][0], a[1][0], a[0][1], a[1][1], t0, t1);
-                        mma(o[z][g][1], a[2][0], a[3][0], a[2][1], a[3][1], t0, t1);
+                        mma(o[z][g][0], a[0][0], a[1][0], a[0][1], a[1][1], b0[k], b1[k]);
+                        mma(o[z][g][1], a[2][0], a[3][0], a[2][1], a[3][1], b0[k], b1[k]);
                     }
                 }
             }
         }
+    };
+
+    bool alive = true;
+    int it = 0;
+    for (int blk = my_lo + warp; blk < my_hi; blk += p.warps, ++it) {
+        const int st = it % STAGES;
+        alive = mbar_wait_warp(bar0 + st * 8, (it / STAGES) & 1, failed);
+        if (!alive) {
+            if (lane == 0) prb_set_status(p.status, PRB_S_WAIT_TIMEOUT, 41, blockIdx.x, blk);
+            break;
+        }
+        // (two copies of the work, since a stage without a masked key should not carry what one needs)
+        const int key0 = blk * SK;
+        if (key0 + SK - 1 > pos_lo || (p.window > 0 && key0 <= pos_hi - p.window))
+            work(st, key0, std::true_type());
+        else
+            work(st, key0, std::false_type());
         __syncwarp();                                          // every lane has read the stage
         if (blk + STAGES * p.warps < my_hi) {
             request(blk + STAGES * p.warps, st, ahead);
@@ -507,11 +639,11 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, QN == 1 ? (NG <= 2 ? 4 : 3) : 
 #pragma unroll
     for (int z = 0; z < QN; ++z)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        for (int e = 0; e < EN; ++e) {
             float sum = l[z][e];
 #pragma unroll
             for (int o2 = 4; o2 < 32; o2 <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o2);
-            const int row = 8 * z + 2 * j + e;
+            const int row = EN == 1 ? j : 8 * z + 2 * j + e;
             float* st = mine + row * PART;
             if (n == 0) {
                 st[DP] = m[z][e];
@@ -519,9 +651,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, QN == 1 ? (NG <= 2 ? 4 : 3) : 
             }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                float y = mid[z][g][e];
-#pragma unroll
-                for (int o2 = 4; o2 < 32; o2 <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o2);
+                const float y = __shfl_sync(0xffffffffu, mid[z][e], g * 4 + j);
                 float* at = st + g * 32 + 8 * (n & 3) + 4 * (n >> 2);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
@@ -592,9 +722,9 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, QN == 1 ? (NG <= 2 ? 4 : 3) : 
     if (p.parts > 1) cluster_sync_all();                       // nobody leaves while its state may be read
 }
 
-template <int NG, int QN, typename T, bool FAST> int launch_one(const Args& p, cudaStream_t stream) {
-    using L = Layout<NG, QN>;
-    cudaError_t e = prb_allow_shared<attention_4bit_kernel<NG, QN, T, FAST>>(L::bytes(MAX_WARPS));
+template <int NG, int QN, int EN, typename T, bool FAST> int launch_one(const Args& p, cudaStream_t stream) {
+    using L = Layout<NG, QN, EN>;
+    cudaError_t e = prb_allow_shared<attention_4bit_kernel<NG, QN, EN, T, FAST>>(L::bytes(MAX_WARPS));
     if (e != cudaSuccess) return (int)e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((long)p.n_tiles * p.kv_heads * p.subs * p.parts));
@@ -610,16 +740,17 @@ template <int NG, int QN, typename T, bool FAST> int launch_one(const Args& p, c
     attr[1].val.programmaticStreamSerializationAllowed = prb_small_ctas_early() && prb_pdl_enabled() ? 1 : 0;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, attention_4bit_kernel<NG, QN, T, FAST>, p);
+    e = cudaLaunchKernelEx(&cfg, attention_4bit_kernel<NG, QN, EN, T, FAST>, p);
     return e == cudaSuccess ? 0 : (int)e;
 }
 
 // `p` but for subs, parts, warps and piece is set; rows: the most rows of a tile.
-template <int NG, int QN, typename T> int launch_by(Args p, long rows, int max_context, int parts, cudaStream_t stream) {
+template <int NG, int QN, int EN, typename T> int launch_by(Args p, long rows, int max_context, int parts, cudaStream_t stream) {
     constexpr int sk = stage_keys(NG, QN);
     p.piece = p.page_size % sk == 0 ? sk : p.page_size % 32 == 0 ? 32 : 16;
     if (sk % p.page_size == 0) p.piece = p.page_size;
-    const long subs = (rows + 8 * QN - 1) / (8 * QN), units = (long)p.n_tiles * p.kv_heads * subs;
+    constexpr int most = Layout<NG, QN, EN>::ROWS;
+    const long subs = (rows + most - 1) / most, units = (long)p.n_tiles * p.kv_heads * subs;
     if (units > 0x7fffffffL / MAX_PARTS) return PRB_E_SIZE;
     p.subs = (int)subs;
     p.warps = MAX_WARPS;
@@ -629,7 +760,7 @@ template <int NG, int QN, typename T> int launch_by(Args p, long rows, int max_c
     p.parts = 1;
     while (p.parts < MAX_PARTS && units * p.parts * 2 <= 4L * prb_sm_count() && stages >= p.parts * 2 * p.warps) p.parts *= 2;
     if (parts > 0) p.parts = parts;
-    if (p.piece == sk && p.head_dim == 32 * NG) return launch_one<NG, QN, T, true>(p, stream);
-    return launch_one<NG, QN, T, false>(p, stream);
+    if (p.piece == sk && p.head_dim == 32 * NG) return launch_one<NG, QN, EN, T, true>(p, stream);
+    return launch_one<NG, QN, EN, T, false>(p, stream);
 }
 }  // namespace attn4

@@ -11,16 +11,19 @@
 // largest logit (the lowest index among equals), and the largest logit follows.
 //
 // One launch; a cluster of eight CTAs takes a request, each an eighth of the vocabulary, and they meet through
-// distributed shared memory.  First all rows' maximum and sum of exponentials in 32 bits, one read of the logits from
-// memory, which is what bounds it: 64 requests of 5 rows of 50,257 are 64 MB.  Then the one row that is drawn from, in
-// 64 bits: the border between two tokens moves by the error of a running sum over the whole vocabulary, and in 32 bits
-// one draw in some hundred would fall on the other side.  The row comes from the L2, where the first pass left it.
+// distributed shared memory.  First all rows' maximum and sum of exponentials in 32 bits (or their largest logit), one read
+// of the logits from memory, which is what bounds it: 64 requests of 5 rows of 50,257 are 64 MB.  Then the one row that is
+// drawn from, in 64 bits: the border between two tokens moves by the error of a running sum over the whole vocabulary, and
+// in 32 bits one draw in some hundred would fall on the other side.  The row comes from the L2, where the first pass left
+// it; its exponentials (exp64: 20 operations of 64 bits) are taken once and kept in shared memory where they fit.
+// 256 threads, so that four CTAs fit an SM and the clusters of 64 requests run side by side.
 #include "common.cuh"
 #include "tcgen05.cuh"
 
 namespace {
-constexpr int PARTS = 8, THREADS = 512, WARPS = THREADS / 32;
+constexpr int PARTS = 8, THREADS = 256, WARPS = THREADS / 32;
 constexpr int MAX_ROWS = 32;
+constexpr int KEPT = 8192;                // most exponentials of a CTA's share that are kept (64 KB)
 
 struct VerifyArgs {
     int* tokens;
@@ -41,9 +44,7 @@ struct Shared {
     // a row's (maximum, its index, sum of exponentials) by warp, then of the CTA in place 0
     float top[MAX_ROWS][WARPS], sum[MAX_ROWS][WARPS];
     int index[MAX_ROWS][WARPS];
-    double part[WARPS], total;
-    int last[WARPS];             // the last token of a warp's run that has any weight
-    int last_all;
+    double part[2][WARPS], total[2];          // two sums take turns, so that one can be read while the next is made
 };
 
 __device__ __forceinline__ uint32_t at_rank(const void* p, int rank) {
@@ -77,8 +78,33 @@ __device__ __forceinline__ void better(float& v, int& i, float w, int k) {
     }
 }
 
-__global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS) verify_kernel(const VerifyArgs p) {
+// e^x for x <= 0: x = k ln 2 + r with |r| <= ln 2 / 2, and Taylor's series of e^r to r^13 (what it leaves out is below
+// 2^-57); 0 below e^-700.
+__device__ __forceinline__ double exp64(double x) {
+    const double k = rint(x * 1.4426950408889634);
+    double r = fma(k, -0.6931471805599453, x);
+    r = fma(k, -2.3190468138462996e-17, r);                 // (what ln 2 loses in 64 bits)
+    double y = 1.0 / 6227020800.0;
+    y = fma(y, r, 1.0 / 479001600.0);
+    y = fma(y, r, 1.0 / 39916800.0);
+    y = fma(y, r, 1.0 / 3628800.0);
+    y = fma(y, r, 1.0 / 362880.0);
+    y = fma(y, r, 1.0 / 40320.0);
+    y = fma(y, r, 1.0 / 5040.0);
+    y = fma(y, r, 1.0 / 720.0);
+    y = fma(y, r, 1.0 / 120.0);
+    y = fma(y, r, 1.0 / 24.0);
+    y = fma(y, r, 1.0 / 6.0);
+    y = fma(y, r, 0.5);
+    y = fma(y, r, 1.0);
+    y = fma(y, r, 1.0);
+    if (!(x > -700.0)) return 0.0;                          // (-inf, whose r is no number, too)
+    return y * __hiloint2double((1023 + (int)k) << 20, 0);
+}
+
+__global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, 4) verify_kernel(const VerifyArgs p) {
     __shared__ Shared s;
+    extern __shared__ double kept_e[];       // [each] exponentials of the row that is drawn from
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int req = blockIdx.x / PARTS, rank = blockIdx.x % PARTS;
     prb_grid_launch_dependents();
@@ -103,35 +129,45 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS) verify_
         const float* x = p.logits + (long)(r0 + r) * p.logits_stride;
         float top = -INFINITY, sum = 0.0f;
         int index = 0x7fffffff;
-        auto take = [&](const float (&v)[4], const int (&k)[4], int n) {
+        auto take = [&](const float* v, int n, int first) {          // n logits, of the tokens first, first + 1, ..
+            if (greedy) {
+#pragma unroll
+                for (int i = 0; i < n; ++i) better(top, index, v[i], first + i);
+                return;
+            }
             float now = top;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (i < n && (v[i] > now || (index == 0x7fffffff && i == 0))) {
-                    now = v[i];
-                    index = k[i];
-                }
-            if (!greedy) {
-                const float ref = now == -INFINITY ? 0.0f : now;
-                sum *= exp2f((top - ref) * scale);
+            for (int i = 0; i < n; ++i) now = fmaxf(now, v[i]);
+            const float ref = now == -INFINITY ? 0.0f : now;
+            sum *= exp2f((top - ref) * scale);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (i < n) sum += exp2f((v[i] - ref) * scale);
-            }
+            for (int i = 0; i < n; ++i) sum += exp2f((v[i] - ref) * scale);
             top = now;
         };
-        // (a thread's tokens go up, so the first of equals is kept)
-        for (int i = lo + threadIdx.x; i < hi; i += 4 * THREADS) {
-            float v[4];
-            int k[4], n = 0;
+        // 16 bytes at a time from the first such border on; up to three logits before it and behind the last one alone
+        const int head = min((int)((16 - ((uintptr_t)(x + lo) & 15)) & 15) / 4, hi - lo);
+        const int vecs = (hi - lo - head) / 4, tail = lo + head + 4 * vecs;
+        const float4* body = reinterpret_cast<const float4*>(x + lo + head);
+        for (int i = threadIdx.x; i < vecs; i += 4 * THREADS) {
+            float v[16];
+            int n = 0;
 #pragma unroll
-            for (int z = 0; z < 4; ++z) {
-                k[z] = i + z * THREADS;
-                v[z] = k[z] < hi ? x[k[z]] : 0.0f;
-                n += k[z] < hi;
+            for (int k = 0; k < 4; ++k)
+                if (i + k * THREADS < vecs) {
+                    const float4 w = body[i + k * THREADS];
+                    v[4 * k] = w.x; v[4 * k + 1] = w.y; v[4 * k + 2] = w.z; v[4 * k + 3] = w.w;
+                    n = k + 1;
+                }
+            if (n == 4 && !greedy) {
+                take(v, 16, 0);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (k < n) take(v + 4 * k, 4, lo + head + 4 * (i + k * THREADS));
             }
-            take(v, k, n);
         }
+        const int lone = threadIdx.x < 4 ? (threadIdx.x < head ? lo + threadIdx.x : hi) : tail + threadIdx.x - 4;
+        if (threadIdx.x < 8 && lone < hi) take(x + lone, 1, lone);
         // the warp's lanes
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
@@ -196,7 +232,7 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS) verify_
             } else if (greedy) {
                 stays = x == best;
             } else {
-                const double mine = exp(((double)p.logits[(long)(r0 + lane) * p.logits_stride + x] - (double)ref) / (double)t);
+                const double mine = exp64(((double)p.logits[(long)(r0 + lane) * p.logits_stride + x] - (double)ref) / (double)t);
                 const double theirs = p.draft_probs ? (double)p.draft_probs[(long)(r0 + lane) * p.probs_stride + x] : 1.0;
                 stays = (double)p.uniforms[2 * (r0 + lane)] * theirs * (double)sum < mine;
             }
@@ -218,27 +254,34 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS) verify_
         const int run = (hi - lo + WARPS - 1) / WARPS;
         const int w0 = min(lo + warp * run, hi), w1 = min(w0 + run, hi);
         // the CTA's sum, then all CTAs'
+        int turn = 1;
         auto meet = [&](double v) -> double {
+            turn ^= 1;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            cluster_sync_all();                                           // (the last meeting's sums are read)
-            if (lane == 0) s.part[warp] = v;
+            if (lane == 0) s.part[turn][warp] = v;
             __syncthreads();
             if (threadIdx.x == 0) {
                 double a = 0.0;
-                for (int w = 0; w < WARPS; ++w) a += s.part[w];
-                s.total = a;
+                for (int w = 0; w < WARPS; ++w) a += s.part[turn][w];
+                s.total[turn] = a;
             }
             cluster_sync_all();
             double all = 0.0;
-            for (int z = 0; z < PARTS; ++z) all += peer_d(&s.total, z);
+            for (int c = 0; c < PARTS; ++c) all += peer_d(&s.total[turn], c);
             return all;
         };
+        const bool keep = each <= KEPT;
+        auto raw = [&](int i) -> double { return exp64(((double)x[i] - (double)top) * inverse); };
         double z = 0.0;
-        for (int i = w0 + lane; i < w1; i += 32) z += exp(((double)x[i] - (double)top) * inverse);
-        z = meet(z);
+        for (int i = w0 + lane; i < w1; i += 32) {
+            const double e = raw(i);
+            if (keep) kept_e[i - lo] = e;
+            z += e;
+        }
+        z = 1.0 / meet(z);
         auto weight = [&](int i, bool less) -> double {
-            const double w = exp(((double)x[i] - (double)top) * inverse) / z;
+            const double w = (keep ? kept_e[i - lo] : raw(i)) * z;
             if (!less) return w;
             if (q != nullptr) return fmax(w - (double)q[i], 0.0);
             return i == gone ? 0.0 : w;
@@ -258,7 +301,7 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS) verify_
         int owner = -1, final_owner = 0;
         double owner_before = 0.0;
         for (int c = 0; c < PARTS; ++c) {
-            const double v = peer_d(&s.total, c);
+            const double v = peer_d(&s.total[turn], c);
             if (v > 0.0) final_owner = c;
             if (owner < 0 && before + v > want) {
                 owner = c;
@@ -273,7 +316,7 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS) verify_
             int mine = -1, final_mine = 0;
             double mine_before = 0.0;
             for (int w = 0; w < WARPS; ++w) {
-                const double v = s.part[w];
+                const double v = s.part[turn][w];
                 if (v > 0.0) final_mine = w;
                 if (mine < 0 && passes && b + v > want) {
                     mine = w;
@@ -324,6 +367,10 @@ PRB_API int prb_verify_drafts(int* tokens, int* accepted, const float* logits, l
     if (vocab <= 0 || n_requests > 0x7fffffff / PARTS) return PRB_E_SIZE;
     const VerifyArgs a{tokens, accepted, logits, logits_stride, row_start, drafted, draft_probs, probs_stride, uniforms,
                        temperature, n_requests, n_rows, vocab, status};
-    const cudaError_t e = prb_launch_dependent(verify_kernel, dim3((unsigned)n_requests * PARTS), dim3(THREADS), 0, stream, a);
+    const int each = (vocab + PARTS - 1) / PARTS;
+    cudaError_t e = prb_allow_shared<verify_kernel>(KEPT * (int)sizeof(double));
+    if (e != cudaSuccess) return (int)e;
+    e = prb_launch_dependent(verify_kernel, dim3((unsigned)n_requests * PARTS), dim3(THREADS),
+                             each <= KEPT ? each * sizeof(double) : 0, stream, a);
     return e == cudaSuccess ? 0 : (int)e;
 }

@@ -168,14 +168,14 @@ def tiles_of(lengths: Sequence[int], most: int):
 
 
 def attention_bound(ref, terms, keys: int, dtype) -> torch.Tensor:
-    """How far a result may be from the 64-bit one.  bfloat16: half a step of the result (2^-8), and of every
-    probability times its step (2^-8 of A).  Both types: a score that 32-bit sums moved by E moves a probability by up
+    """How far a result may be from the 64-bit one.  bfloat16: half a step of the result (2^-8), of every probability
+    times its step (2^-8 of A) and of every probability that goes with a middle (2^-8 of B - A), so 2^-8 of B.  Both types: a score that 32-bit sums moved by E moves a probability by up
     to 2 E of itself (once by itself, once by the sum of all; e^x - 1 <= 1.01 x here), the exponential is good for
     2^-21 with its argument's rounding (2^-24 of up to 64 log2 units), and sums over the keys one after the other lose up
     to 2^-23 a key."""
-    a, b, e = terms
+    _a, b, e = terms
     assert float(e.max()) < 0.01
     wide = 2 * (1.01 * e + 2.0 ** -21 + 2.0 ** -17) + (keys + 16) * 2.0 ** -23
     if dtype == torch.float32:
         return wide * b + 2.0 ** -23 * ref.abs() + 1e-30
-    return 1.01 * 2.0 ** -8 * (ref.abs() + a) + wide * b + 1e-30
+    return 1.01 * 2.0 ** -8 * (ref.abs() + b) + wide * b + 1e-30
