@@ -51,12 +51,14 @@ def load_lm(path: str, opts: Optional[Dict] = None, *, gpu: bool = True,
             dtype: str = "bfloat16", device_id: str = "cuda:0", maxpos: Optional[int] = None,
             page_size: int = 64, max_lanes: int = 64, max_batched_tokens: int = 2048,
             prefill_chunk: int = 512, max_tokens: Optional[int] = None,
-            share_prefixes: bool = True) -> LM:
+            share_prefixes: bool = True, cache_bits: Optional[int] = None) -> LM:
     """Load the model folder ``path`` (``config.json`` + ``model.safetensors``); the model
     class is chosen by ``config.json``.  Options, by the reference's names where it has
     them (``lm.clj:94-115``): ``gpu`` (must be true), ``device_id``, ``maxpos``: the most
-    tokens a request may hold (default and upper bound: the model's positions).  ``opts``
-    may give the same options as a dict (``{"gpu?": True, "maxpos": 2048}``)."""
+    tokens a request may hold (default and upper bound: the model's positions).  ``cache_bits=4``
+    caches keys and values in 4 bits (GPT-2): a third of the cache's memory and traffic, at
+    the price of their rounding.  ``opts`` may give the same options as a dict (``{"gpu?":
+    True, "maxpos": 2048}``)."""
     from .engine.engine import Engine
     from .engine.loading import load_model
     from .engine.scheduler import SchedulerOptions
@@ -65,6 +67,7 @@ def load_lm(path: str, opts: Optional[Dict] = None, *, gpu: bool = True,
         device_id = opts.get("device-id", opts.get("device_id", device_id))
         maxpos = opts.get("maxpos", maxpos)
         dtype = opts.get("dtype", dtype)
+        cache_bits = opts.get("cache-bits", opts.get("cache_bits", cache_bits))
     if not gpu:
         raise ValueError("pretrained_rstr_b200 has no CPU path: load_lm(..., gpu=True) only")
     from .config.registry import read_config
@@ -76,7 +79,7 @@ def load_lm(path: str, opts: Optional[Dict] = None, *, gpu: bool = True,
         max_tokens = max_lanes * (-(-per_request // page_size) * page_size)
     loaded = load_model(path, dtype=dtype, device=device_id, page_size=page_size,
                         max_batched_tokens=max_batched_tokens, max_requests=max_lanes,
-                        max_tokens=max_tokens, share_prefixes=share_prefixes)
+                        max_tokens=max_tokens, share_prefixes=share_prefixes, cache_bits=cache_bits)
     engine = Engine(loaded, SchedulerOptions(
         max_batched_tokens=max_batched_tokens, max_lanes=max_lanes,
         prefill_chunk=min(prefill_chunk, max_batched_tokens),

@@ -26,7 +26,7 @@ def _generate(args) -> int:
     with random_model_folder(args.random, args.weights_seed, args.dtype) if args.random \
             else contextlib.nullcontext(args.model) as folder:
         m = load_lm(folder, gpu=args.gpu, dtype=args.dtype, device_id=args.device_id,
-                    maxpos=args.maxpos, max_lanes=args.max_lanes)
+                    maxpos=args.maxpos, max_lanes=args.max_lanes, cache_bits=args.cache_bits)
     opts = {}
     if args.temperature is not None:
         opts = {"temperature": args.temperature, "top_k": args.top_k, "top_p": args.top_p,
@@ -87,6 +87,7 @@ def main(argv=None) -> int:
     g.add_argument("--device-id", default="cuda:0")
     g.add_argument("--maxpos", type=int, default=None)
     g.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    g.add_argument("--cache-bits", type=int, default=None, choices=[4], help="cache keys and values in 4 bits (GPT-2)")
     g.add_argument("--max-lanes", type=int, default=4)
     g.set_defaults(fn=_generate)
     r = sub.add_parser("random", help="write a model folder with seeded random weights")

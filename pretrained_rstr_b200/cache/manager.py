@@ -59,6 +59,7 @@ class GroupSpec:
     head_dim: int
     window: Optional[int] = None
     pools_per_layer: int = 2          # keys and values; 1: one row per token serves as both
+    bits: Optional[int] = None        # 4: pages held in 4 bits; None: in the runtime's type
 
     @property
     def elements_per_token(self) -> int:

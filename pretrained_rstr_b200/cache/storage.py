@@ -5,7 +5,9 @@ Pages of a group: one tensor ``[pools, pages, kv_heads, page_size, head_dim]`` w
 one row per token as key and value has one pool per layer), so one page id
 addresses every layer of the group (``src/pretrained/continuation/page_pool.clj:4-6``)
 and a page of one (layer, head) is one contiguous tile.  Element type: the runtime's
-(bfloat16 when serving, float32 on the 32-bit path).
+(bfloat16 when serving, float32 on the 32-bit path).  A group held in 4 bits is uint8
+``[pools, pages, kv_heads, bytes of a tile]`` (``ops.cache4_tile_bytes``): codes of a page's
+rows, then their steps and middles, 0.31 of bfloat16's bytes at head size 64.
 
 State: one tensor ``[slots, *shape]`` per (layer, name) a mixer declared, zero-filled.
 """
@@ -28,8 +30,13 @@ class CacheStorage:
         self.num_pages = list(num_pages)
         self.kv: List[torch.Tensor] = []
         for g, n in zip(self.groups, self.num_pages):
-            self.kv.append(torch.zeros((g.pools_per_layer * len(g.layers), n, g.kv_heads, page_size,
-                                        g.head_dim), dtype=dtype, device=device))
+            pools = g.pools_per_layer * len(g.layers)
+            if g.bits == 4:
+                self.kv.append(torch.zeros((pools, n, g.kv_heads, ops.cache4_tile_bytes(g.head_dim, page_size)),
+                                           dtype=torch.uint8, device=device))
+            else:
+                self.kv.append(torch.zeros((pools, n, g.kv_heads, page_size, g.head_dim), dtype=dtype,
+                                           device=device))
         self.state: Dict[Tuple[int, str], torch.Tensor] = {
             key: torch.zeros((num_slots,) + tuple(spec.shape), dtype=spec.dtype, device=device)
             for key, spec in state_specs.items()}

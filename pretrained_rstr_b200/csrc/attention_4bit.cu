@@ -41,7 +41,7 @@ PRB_API int prb_attention_4bit(void* out, long out_stride, const void* q, long q
     p.k_tiles = (const uint8_t*)k_tiles; p.v_tiles = (const uint8_t*)v_tiles;
     p.block_table = block_table; p.positions = positions;
     p.tile_req = tile_req; p.tile_row0 = tile_row0; p.tile_rows = tile_rows; p.tile_count = tile_count;
-    p.n_tokens = n_tokens; p.n_requests = n_requests; p.n_tiles = n_tiles;
+    p.n_tokens = n_tokens; p.n_requests = n_requests; p.n_tiles = n_tiles; p.tile_most = tile_most;
     p.heads = heads; p.kv_heads = kv_heads; p.hpg = hpg;
     p.head_dim = head_dim; p.page_size = page_size;
     p.max_pages = max_pages; p.num_pages = num_pages;

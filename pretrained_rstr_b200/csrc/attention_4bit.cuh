@@ -57,7 +57,7 @@ struct Args {
     const int* tile_count;                 // null: every tile of the launch
     int n_tokens;                          // rows of q and out
     int n_requests;                        // rows of the block table
-    int n_tiles, subs, parts, warps;
+    int n_tiles, tile_most, subs, parts, warps;
     int heads, kv_heads, hpg;              // hpg: query heads per key/value head
     int head_dim, page_size, piece;        // piece: keys that lie together in a page and in a stage
     int max_pages, num_pages;
@@ -754,9 +754,10 @@ template <int NG, int QN, int EN, typename T> int launch_by(Args p, long rows, i
     if (units > 0x7fffffffL / MAX_PARTS) return PRB_E_SIZE;
     p.subs = (int)subs;
     p.warps = MAX_WARPS;
-    // Parts of a unit's keys: as many as give every SM about four CTAs, each with a stage a warp at least.
-    const int span = p.window > 0 && p.window < max_context ? p.window + sk : max_context;
-    const int stages = (span + sk - 1) / sk;
+    // Parts of a unit's keys: as many as give every SM about four CTAs, each with a stage a warp at least.  (The longest
+    // request's: max_context, or what a window and the tile's own tokens span.)
+    const int reach = p.window > 0 ? min((long)max_context, (long)p.window + p.tile_most + sk) : max_context;
+    const int stages = (reach + sk - 1) / sk + (p.window > 0 ? 1 : 0);   // (a window need not begin with a stage)
     p.parts = 1;
     while (p.parts < MAX_PARTS && units * p.parts * 2 <= 4L * prb_sm_count() && stages >= p.parts * 2 * p.warps) p.parts *= 2;
     if (parts > 0) p.parts = parts;

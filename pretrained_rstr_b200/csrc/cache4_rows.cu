@@ -1,7 +1,8 @@
 // Rows of keys and values into a cache held in 4 bits, and back (cache4.cuh has the layout).
 //
-// Both kernels are bound by memory, or by their launch for a few tokens: 2,048 tokens of 25 heads of 64 read
-// 13 MB of bfloat16 and write 4 MB.  Four threads share a group of 32 channels, 8 channels (16 bytes of
+// A decode step's 64 tokens of 12 heads of 64 are bound by the launch (2.5 us in, 2.0 us back).  2,048 tokens of 25 heads
+// go in at 12.7 us, bound by the instructions of the rounding (17 MB move, 2.6 us' worth), and back at 8.6 us (30 MB, 4.6 us'
+// worth).  Four threads share a group of 32 channels, 8 channels (16 bytes of
 // bfloat16, one 32-bit word of codes) each; neighbouring threads take neighbouring groups of one token, so a
 // warp reads 512 bytes in a row.  The smallest and the largest number of a group meet in two shuffles.
 //
@@ -68,18 +69,21 @@ __device__ __forceinline__ uint32_t code_of(float x, float middle, float step, f
     return static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(n, -8.0f), 7.0f)) + 8);
 }
 
+// The slot of a token, or -1: it has none (recorded where it lies outside the pool).
+__device__ __forceinline__ int slot_of(const RowArgs& a, int token) {
+    const int slot = a.slots[token];
+    if (slot < a.num_pages * a.page_size) return slot;
+    if (threadIdx.x == 0 && blockIdx.y == 0) prb_set_status(a.status, PRB_S_SLOT_RANGE, token, slot, a.num_pages);
+    return -1;
+}
+
+// (Several tokens a CTA, all asked for first, measured no faster for keys coming in and slower for those going back.)
 template <typename T>
 __global__ void __launch_bounds__(256) kv_append_4bit_kernel(RowArgs a, int wide) {
     prb_grid_launch_dependents();
     prb_grid_wait();
-    const int token = blockIdx.x;
-    const int slot = a.slots[token];
-    if (slot < 0) return;
-    if (slot >= a.num_pages * a.page_size) {
-        if (threadIdx.x == 0 && blockIdx.y == 0) prb_set_status(a.status, PRB_S_SLOT_RANGE, token, slot, a.num_pages);
-        return;
-    }
-    const int page = slot / a.page_size, at = slot - page * a.page_size;
+    const int token = blockIdx.x, slot = slot_of(a, token);
+    if (slot < 0) return;                               // (the whole CTA)
     const int per = a.heads * a.groups;                 // groups of a token's keys (and of its values)
     const int quarter = threadIdx.x & 3;
     const int unit = (blockIdx.y * blockDim.x + threadIdx.x) >> 2;
@@ -123,6 +127,7 @@ __global__ void __launch_bounds__(256) kv_append_4bit_kernel(RowArgs a, int wide
 #pragma unroll
         for (int i = 0; i < 8; ++i) word |= code_of(x[i], middle, step, inverse) << (4 * i);
     }
+    const int page = slot / a.page_size, at = slot - page * a.page_size;
     uint8_t* tile = (kind ? a.tiles[1] : a.tiles[0]) +
                     ((size_t)page * a.heads + head) * (size_t)cache4::tile_bytes(a.head_dim, a.page_size);
     *reinterpret_cast<uint32_t*>(tile + cache4::code_word(a.head_dim, a.page_size, at, channel / 8)) = word;
@@ -137,17 +142,12 @@ template <typename T>
 __global__ void __launch_bounds__(256) kv_read_4bit_kernel(RowArgs a, int wide) {
     prb_grid_launch_dependents();
     prb_grid_wait();
-    const int token = blockIdx.x;
-    const int slot = a.slots[token];
+    const int token = blockIdx.x, slot = slot_of(a, token);
     if (slot < 0) return;
-    if (slot >= a.num_pages * a.page_size) {
-        if (threadIdx.x == 0 && blockIdx.y == 0) prb_set_status(a.status, PRB_S_SLOT_RANGE, token, slot, a.num_pages);
-        return;
-    }
-    const int page = slot / a.page_size, at = slot - page * a.page_size;
     const int words = a.head_dim / 8, per = a.heads * words;
     const int unit = blockIdx.y * blockDim.x + threadIdx.x;
     if (unit >= 2 * per) return;
+    const int page = slot / a.page_size, at = slot - page * a.page_size;
     const int kind = unit >= per ? 1 : 0, hw = unit - kind * per;
     const int head = hw / words, w = hw - head * words;
     const uint8_t* tile = (kind ? a.tiles[1] : a.tiles[0]) +
@@ -183,8 +183,9 @@ int launch_rows(bool append, RowArgs a, int dtype, cudaStream_t stream) {
     }
     a.groups = cache4::groups_of(a.head_dim);
     const int threads_of_token = append ? 2 * a.heads * a.groups * 4 : 2 * a.heads * (a.head_dim / 8);
-    const int threads = threads_of_token >= 256 ? 256 : ((threads_of_token + 31) / 32) * 32;
-    const dim3 grid(a.n_tokens, (threads_of_token + threads - 1) / threads);
+    // (as few CTAs a token as its threads need, of equal size)
+    const int blocks = (threads_of_token + 255) / 256, threads = ((threads_of_token + blocks - 1) / blocks + 31) / 32 * 32;
+    const dim3 grid(a.n_tokens, blocks);
     cudaError_t e;
     if (append)
         e = dtype == PRB_F32

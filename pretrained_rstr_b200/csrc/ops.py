@@ -2685,25 +2685,27 @@ STEP_TABLES_MAX_REQUESTS = 4096         # most requests of a step that step_tabl
 VERIFY_DRAFTS_MAX_TOKENS = 31           # most drafted tokens of a request that verify_drafts takes
 
 
-def _one_device(what: str, names, tensors) -> int:
-    """The CUDA device that all of ``tensors`` (None is skipped) lie on."""
-    device = None
-    for i, t in enumerate(tensors):
-        if t is None:
+_U8, _I32, _F32 = torch.uint8, torch.int32, torch.float32
+_CODES = {torch.float32: F32, torch.bfloat16: BF16}
+
+
+def _elsewhere(what: str, names: str, *tensors):
+    """The tensors do not lie on one CUDA device: says which."""
+    first = None
+    for name, t in zip(names.split(), tensors):
+        d = None if t is None else t.get_device()
+        if d is None or d == first:
             continue
-        d = t.get_device()
-        if d != device:
-            if d < 0:
-                raise KernelArgumentError(f"{what}: {names.split()[i]} is not on a CUDA device")
-            if device is not None:
-                raise KernelArgumentError(f"{what}: {names.split()[i]} is on device {d}, the others on device {device}")
-            device = d
-    return device
+        if d < 0:
+            raise KernelArgumentError(f"{what}: {name} is not on a CUDA device")
+        if first is not None:
+            raise KernelArgumentError(f"{what}: {name} is on device {d}, the others on device {first}")
+        first = d
 
 
 def _launch_on(device: int, what: str, name: str, *args) -> None:
     """The library's ``name(*args, stream)`` on ``device``'s current stream, whatever the current device is."""
-    call = getattr(lib(), name)
+    call = getattr(_LIB or lib(), name)
     if device == torch._C._cuda_getDevice():
         code = call(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
@@ -2714,22 +2716,32 @@ def _launch_on(device: int, what: str, name: str, *args) -> None:
 
 def _ints(what: str, name: str, t, n: int) -> int:
     """The address of a contiguous int32 tensor of at least ``n`` numbers."""
-    if t.dtype is not torch.int32 or t.numel() < n or not t.is_contiguous():
+    if t.dtype is not _I32 or t.numel() < n or not t.is_contiguous():
         raise KernelArgumentError(f"{what}: {name} must be contiguous int32 with at least {n} numbers, is "
                                   f"{t.dtype} {list(t.shape)}")
     return t.data_ptr()
 
 
-def _status4(what: str, status):
-    return None if status is None else _ints(what, "status", status, 4)
-
-
 def _matrix4(what: str, name: str, t, rows: int, width: int) -> int:
-    """The element type's code of [>= rows, width] with neighbouring columns."""
-    if t.dim() != 2 or t.shape[1] != width or t.shape[0] < rows or (width > 1 and t.stride(1) != 1) or t.stride(0) < 0:
+    """The row stride of [>= rows, width] with neighbouring columns."""
+    if t.dim() != 2:
+        raise KernelArgumentError(f"{what}: {name} must be [tokens, {width}], is {list(t.shape)}")
+    n, w = t.shape
+    stride, step = t.stride()
+    if w != width or n < rows or (step != 1 and width > 1) or stride < 0:
         raise KernelArgumentError(f"{what}: {name} must be [tokens, {width}] with neighbouring columns and at least "
                                   f"{rows} rows, is {list(t.shape)}")
-    return dtype_code(t.dtype)
+    return stride
+
+
+def _code4(what: str, a_name: str, b_name: str, a, b) -> int:
+    """The code of the two tensors' one element type."""
+    code = _CODES.get(a.dtype)
+    if code is None:
+        return dtype_code(a.dtype)                          # (refuses it)
+    if b.dtype is not a.dtype:
+        raise KernelArgumentError(f"{what}: {a_name} and {b_name} differ in type")
+    return code
 
 
 def cache4_tile_bytes(head_dim: int, page_size: int) -> int:
@@ -2743,32 +2755,21 @@ def cache4_tile_bytes(head_dim: int, page_size: int) -> int:
     return page_size * (head_dim // 2 + 4 * ((head_dim + 31) // 32))
 
 
+_TILE_BYTES = {}                        # (head size, page size) -> bytes of a tile
+
+
 def _tiles4(what: str, k_tiles, v_tiles, head_dim: int, page_size: int):
-    tile = cache4_tile_bytes(head_dim, page_size)
-    for name, t in (("k_tiles", k_tiles), ("v_tiles", v_tiles)):
-        if t.dtype is not torch.uint8 or t.dim() != 3 or t.shape[2] != tile or not t.is_contiguous():
-            raise KernelArgumentError(f"{what}: {name} must be contiguous uint8 [pages, heads, {tile}], is {t.dtype} "
-                                      f"{list(t.shape)}")
-    pages, heads, _tile = k_tiles.shape
-    if v_tiles.shape[0] != pages or v_tiles.shape[1] != heads:
-        raise KernelArgumentError(f"{what}: k_tiles and v_tiles differ in shape")
-    return pages, heads
-
-
-def _rows_4bit(what: str, call, first: bool, names, a, b, k_tiles, v_tiles, slots, n_tokens, head_dim, page_size, status):
-    device = _one_device(what, names + " k_tiles v_tiles slots status", (a, b, k_tiles, v_tiles, slots, status))
-    pages, heads = _tiles4(what, k_tiles, v_tiles, head_dim, page_size)
-    if n_tokens < 0:
-        raise KernelArgumentError(f"{what}: n_tokens is below zero")
-    a_name, b_name = names.split()
-    code = _matrix4(what, a_name, a, n_tokens, heads * head_dim)
-    if _matrix4(what, b_name, b, n_tokens, heads * head_dim) != code:
-        raise KernelArgumentError(f"{what}: {a_name} and {b_name} differ in type")
-    rows = (a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0))
-    tiles = (k_tiles.data_ptr(), v_tiles.data_ptr())
-    slots, status = _ints(what, "slots", slots, n_tokens), _status4(what, status)
-    _launch_on(device, what, call, *(tiles + rows if first else rows + tiles), slots, n_tokens, heads,
-               head_dim, page_size, pages, code, status)
+    tile = _TILE_BYTES.get((head_dim, page_size))
+    if tile is None:
+        tile = _TILE_BYTES[(head_dim, page_size)] = cache4_tile_bytes(head_dim, page_size)
+    shape = k_tiles.shape
+    if len(shape) != 3 or shape[2] != tile or k_tiles.dtype is not _U8 or not k_tiles.is_contiguous():
+        raise KernelArgumentError(f"{what}: k_tiles must be contiguous uint8 [pages, heads, {tile}], is {k_tiles.dtype} "
+                                  f"{list(shape)}")
+    if v_tiles.shape != shape or v_tiles.dtype is not _U8 or not v_tiles.is_contiguous():
+        raise KernelArgumentError(f"{what}: k_tiles and v_tiles differ in shape, type or layout: {list(shape)}, "
+                                  f"{v_tiles.dtype} {list(v_tiles.shape)}")
+    return shape
 
 
 def kv_append_4bit(k_tiles, v_tiles, k, v, slots, n_tokens: int, head_dim: int, page_size: int, status) -> None:
@@ -2781,16 +2782,40 @@ def kv_append_4bit(k_tiles, v_tiles, k, v, slots, n_tokens: int, head_dim: int, 
     smallest + 8 step in bfloat16 and per channel the nearest of 16 codes; code c reads back as middle + step * (c - 8).
     A group whose step would be below 2^-126 reads back as its smallest number; one that holds an infinity or a NaN
     reads back as NaN."""
-    _rows_4bit("kv_append_4bit", "prb_kv_append_4bit", True, "k v", k, v, k_tiles, v_tiles, slots, n_tokens, head_dim,
-               page_size, status)
+    what = "kv_append_4bit"
+    device = k_tiles.get_device()
+    if device < 0 or v_tiles.get_device() != device or k.get_device() != device or v.get_device() != device or \
+            slots.get_device() != device or (status is not None and status.get_device() != device):
+        _elsewhere(what, "k_tiles v_tiles k v slots status", k_tiles, v_tiles, k, v, slots, status)
+    pages, heads, _tile = _tiles4(what, k_tiles, v_tiles, head_dim, page_size)
+    if n_tokens < 0:
+        raise KernelArgumentError(f"{what}: n_tokens is below zero")
+    width = heads * head_dim
+    k_stride, v_stride = _matrix4(what, "k", k, n_tokens, width), _matrix4(what, "v", v, n_tokens, width)
+    _launch_on(device, what, "prb_kv_append_4bit", k_tiles.data_ptr(), v_tiles.data_ptr(), k.data_ptr(), k_stride,
+               v.data_ptr(), v_stride, _ints(what, "slots", slots, n_tokens), n_tokens, heads, head_dim, page_size, pages,
+               _code4(what, "k", "v", k, v), None if status is None else _ints(what, "status", status, 4))
 
 
 def kv_read_4bit(k_out, v_out, k_tiles, v_tiles, slots, n_tokens: int, head_dim: int, page_size: int, status) -> None:
     """What a cache held in 4 bits stands for at ``slots`` (see :func:`kv_append_4bit`): rows of ``k_out`` / ``v_out``
     [T, kv_heads * head_dim], float32 (exact but for a last rounding to 32 bits) or bfloat16.  Rows whose slot is below
     zero stay as they were."""
-    _rows_4bit("kv_read_4bit", "prb_kv_read_4bit", False, "k_out v_out", k_out, v_out, k_tiles, v_tiles, slots, n_tokens,
-               head_dim, page_size, status)
+    what = "kv_read_4bit"
+    device = k_tiles.get_device()
+    if device < 0 or v_tiles.get_device() != device or k_out.get_device() != device or v_out.get_device() != device or \
+            slots.get_device() != device or (status is not None and status.get_device() != device):
+        _elsewhere(what, "k_tiles v_tiles k_out v_out slots status", k_tiles, v_tiles, k_out, v_out, slots, status)
+    pages, heads, _tile = _tiles4(what, k_tiles, v_tiles, head_dim, page_size)
+    if n_tokens < 0:
+        raise KernelArgumentError(f"{what}: n_tokens is below zero")
+    width = heads * head_dim
+    k_stride = _matrix4(what, "k_out", k_out, n_tokens, width)
+    v_stride = _matrix4(what, "v_out", v_out, n_tokens, width)
+    _launch_on(device, what, "prb_kv_read_4bit", k_out.data_ptr(), k_stride, v_out.data_ptr(), v_stride,
+               k_tiles.data_ptr(), v_tiles.data_ptr(), _ints(what, "slots", slots, n_tokens), n_tokens, heads, head_dim,
+               page_size, pages, _code4(what, "k_out", "v_out", k_out, v_out),
+               None if status is None else _ints(what, "status", status, 4))
 
 
 def attention_4bit(out, q, k_tiles, v_tiles, block_table, positions, tile_req, tile_row0, tile_rows, tile_most: int,
@@ -2808,23 +2833,30 @@ def attention_4bit(out, q, k_tiles, v_tiles, block_table, positions, tile_req, t
     positions only.  ``max_context``: the most positions a request holds (the keys are cut into parts by it).
     ``parts``: CTAs that share a tile's keys (0: the kernel's rule).  Rows of no tile stay as they were."""
     what = "attention_4bit"
-    device = _one_device(what, "out q k_tiles v_tiles block_table positions tile_req tile_row0 tile_rows tile_count status",
-                         (out, q, k_tiles, v_tiles, block_table, positions, tile_req, tile_row0, tile_rows, tile_count,
-                          status))
-    pages, kv_heads = _tiles4(what, k_tiles, v_tiles, head_dim, page_size)
+    device = q.get_device()
+    if device < 0 or out.get_device() != device or k_tiles.get_device() != device or v_tiles.get_device() != device or \
+            block_table.get_device() != device or positions.get_device() != device or tile_req.get_device() != device or \
+            tile_row0.get_device() != device or tile_rows.get_device() != device or \
+            (tile_count is not None and tile_count.get_device() != device) or \
+            (status is not None and status.get_device() != device):
+        _elsewhere(what, "q out k_tiles v_tiles block_table positions tile_req tile_row0 tile_rows tile_count status", q, out,
+                   k_tiles, v_tiles, block_table, positions, tile_req, tile_row0, tile_rows, tile_count, status)
+    pages, kv_heads, _tile = _tiles4(what, k_tiles, v_tiles, head_dim, page_size)
     if n_heads < 1 or n_heads % kv_heads:
         raise KernelArgumentError(f"{what}: {n_heads} query heads are not a multiple of {kv_heads} key/value heads")
-    if window is not None and window < 1:
+    if window is None:
+        window = 0
+    elif window < 1:
         raise KernelArgumentError(f"{what}: a window holds at least the token itself")
     if tile_most < 1 or max_context < 1 or not 0 <= parts <= ATTENTION_4BIT_MAX_PARTS or not math.isfinite(scale):
         raise KernelArgumentError(f"{what}: tile_most and max_context are at least 1, parts 0 to "
                                   f"{ATTENTION_4BIT_MAX_PARTS}, scale is finite; got {tile_most}, {max_context}, {parts}, "
                                   f"{scale}")
     width = n_heads * head_dim
+    q_stride = _matrix4(what, "q", q, 0, width)
     tokens = q.shape[0]
-    code = _matrix4(what, "q", q, 0, width)
-    if _matrix4(what, "out", out, tokens, width) != code:
-        raise KernelArgumentError(f"{what}: q and out differ in type")
+    out_stride = _matrix4(what, "out", out, tokens, width)
+    code = _code4(what, "q", "out", q, out)
     q_at, out_at = q.data_ptr(), out.data_ptr()
     if q_at == out_at and tokens > 0:
         raise KernelArgumentError(f"{what}: out must not be q")
@@ -2833,13 +2865,13 @@ def attention_4bit(out, q, k_tiles, v_tiles, block_table, positions, tile_req, t
     requests, wide = block_table.shape
     n_tiles = tile_req.numel()
     _launch_on(device, what, "prb_attention_4bit",
-               out_at, out.stride(0), q_at, q.stride(0), k_tiles.data_ptr(), v_tiles.data_ptr(),
+               out_at, out_stride, q_at, q_stride, k_tiles.data_ptr(), v_tiles.data_ptr(),
                _ints(what, "block_table", block_table, 0), _ints(what, "positions", positions, tokens),
                _ints(what, "tile_req", tile_req, 0), _ints(what, "tile_row0", tile_row0, n_tiles),
                _ints(what, "tile_rows", tile_rows, n_tiles),
                None if tile_count is None else _ints(what, "tile_count", tile_count, 1), n_tiles, tile_most, tokens,
-               requests, n_heads, kv_heads, head_dim, page_size, wide, pages, scale, window or 0, max_context, parts, code,
-               _status4(what, status))
+               requests, n_heads, kv_heads, head_dim, page_size, wide, pages, scale, window, max_context, parts, code,
+               None if status is None else _ints(what, "status", status, 4))
 
 
 def step_tables(rows, held, brought, tables, page_size: int, q_start, kv_len, positions, seq_of_token, slots, block_table,
@@ -2852,16 +2884,24 @@ def step_tables(rows, held, brought, tables, page_size: int, q_start, kv_len, po
     ``block_table`` [requests, pages a request]: the request's pages up to its last new token, -1 behind them.  Pages a
     request grows into come from ``free_pages`` [``free_start[0]`` ...], in the requests' order, and are put into
     ``tables`` too; ``free_next[0]`` becomes the place behind the last one taken (not ``free_start`` itself: the caller
-    has the two take turns).  Without ``free_pages`` the rows of ``tables`` hold the pages already (the cache manager
-    reserves them on the host).
+    has the two take turns).  What a row holds behind its request's ``held`` tokens is overwritten, not used: where
+    requests give tokens back (refused drafts), their pages are better reserved beforehand.  Without ``free_pages`` the
+    rows of ``tables`` hold the pages already (the cache manager reserves them on the host).
 
     In the status word: a request whose row or lengths do not fit (it brings nothing, its block table row stays
     empty), a page that is missing (the slot is -1), more tokens than token rows (those behind are left out)."""
     what = "step_tables"
-    device = _one_device(what, "rows held brought tables q_start kv_len positions seq_of_token slots block_table status "
-                         "free_pages free_start free_next",
-                         (rows, held, brought, tables, q_start, kv_len, positions, seq_of_token, slots, block_table, status,
-                          free_pages, free_start, free_next))
+    device = held.get_device()
+    if device < 0 or rows.get_device() != device or brought.get_device() != device or tables.get_device() != device or \
+            q_start.get_device() != device or kv_len.get_device() != device or positions.get_device() != device or \
+            seq_of_token.get_device() != device or slots.get_device() != device or \
+            block_table.get_device() != device or (status is not None and status.get_device() != device) or \
+            (free_pages is not None and free_pages.get_device() != device) or \
+            (free_start is not None and free_start.get_device() != device) or \
+            (free_next is not None and free_next.get_device() != device):
+        _elsewhere(what, "held rows brought tables q_start kv_len positions seq_of_token slots block_table status "
+                   "free_pages free_start free_next", held, rows, brought, tables, q_start, kv_len, positions, seq_of_token,
+                   slots, block_table, status, free_pages, free_start, free_next)
     n, cap = held.numel(), positions.numel()
     if not 1 <= n <= STEP_TABLES_MAX_REQUESTS:
         raise KernelArgumentError(f"{what}: takes 1 to {STEP_TABLES_MAX_REQUESTS} requests, got {n}")
@@ -2887,7 +2927,8 @@ def step_tables(rows, held, brought, tables, page_size: int, q_start, kv_len, po
                _ints(what, "rows", rows, n), _ints(what, "held", held, n), _ints(what, "brought", brought, n), t_at,
                free_at, start_at, next_at, _ints(what, "q_start", q_start, n + 1), _ints(what, "kv_len", kv_len, n),
                _ints(what, "positions", positions, 0), _ints(what, "seq_of_token", seq_of_token, cap),
-               _ints(what, "slots", slots, cap), b_at, n, lanes, cap, wide, page_size, n_free, _status4(what, status))
+               _ints(what, "slots", slots, cap), b_at, n, lanes, cap, wide, page_size, n_free,
+               None if status is None else _ints(what, "status", status, 4))
 
 
 def verify_drafts(tokens, accepted, logits, row_start, drafted, uniforms, temperature, status, draft_probs=None) -> None:
@@ -2906,26 +2947,31 @@ def verify_drafts(tokens, accepted, logits, row_start, drafted, uniforms, temper
     Written: ``accepted[b]``: drafted tokens that stay; ``tokens`` int32 [rows]: they and the token behind them, -1 in
     the request's rows beyond."""
     what = "verify_drafts"
-    device = _one_device(what, "tokens accepted logits row_start drafted uniforms temperature status draft_probs",
-                         (tokens, accepted, logits, row_start, drafted, uniforms, temperature, status, draft_probs))
-    for name, t in (("logits", logits), ("draft_probs", draft_probs)):
-        if t is not None and (t.dtype is not torch.float32 or t.dim() != 2 or t.stride(0) < 0 or
-                              (t.shape[1] > 1 and t.stride(1) != 1)):
-            raise KernelArgumentError(f"{what}: {name} must be float32 [rows, vocabulary] with neighbouring columns")
+    device = logits.get_device()
+    if device < 0 or tokens.get_device() != device or accepted.get_device() != device or \
+            row_start.get_device() != device or drafted.get_device() != device or uniforms.get_device() != device or \
+            temperature.get_device() != device or (status is not None and status.get_device() != device) or \
+            (draft_probs is not None and draft_probs.get_device() != device):
+        _elsewhere(what, "logits tokens accepted row_start drafted uniforms temperature status draft_probs", logits, tokens,
+                   accepted, row_start, drafted, uniforms, temperature, status, draft_probs)
+    if logits.dtype is not _F32 or logits.dim() != 2 or (draft_probs is not None and draft_probs.dtype is not _F32):
+        raise KernelArgumentError(f"{what}: logits and draft_probs must be float32 [rows, vocabulary]")
     rows, vocab = logits.shape
-    if draft_probs is not None and (draft_probs.shape[0] != rows or draft_probs.shape[1] != vocab):
-        raise KernelArgumentError(f"{what}: draft_probs and logits differ in shape")
     if vocab < 1:
         raise KernelArgumentError(f"{what}: an empty vocabulary")
+    l_stride = _matrix4(what, "logits", logits, rows, vocab)
+    p_at, p_stride = None, 0
+    if draft_probs is not None:
+        if draft_probs.shape != logits.shape:
+            raise KernelArgumentError(f"{what}: draft_probs and logits differ in shape")
+        p_at, p_stride = draft_probs.data_ptr(), _matrix4(what, "draft_probs", draft_probs, rows, vocab)
     n = temperature.numel()
     for name, t, k in (("temperature", temperature, n), ("uniforms", uniforms, 2 * rows)):
-        if t.dtype is not torch.float32 or t.numel() < k or not t.is_contiguous():
+        if t.dtype is not _F32 or t.numel() < k or not t.is_contiguous():
             raise KernelArgumentError(f"{what}: {name} must be contiguous float32 with at least {k} numbers")
     tokens_at, drafted_at = _ints(what, "tokens", tokens, rows), _ints(what, "drafted", drafted, rows)
     if tokens_at < drafted_at + 4 * rows and drafted_at < tokens_at + 4 * rows:
         raise KernelArgumentError(f"{what}: tokens and drafted are two tensors")
     _launch_on(device, what, "prb_verify_drafts", tokens_at, _ints(what, "accepted", accepted, n), logits.data_ptr(),
-               logits.stride(0), _ints(what, "row_start", row_start, n + 1), drafted_at,
-               None if draft_probs is None else draft_probs.data_ptr(),
-               0 if draft_probs is None else draft_probs.stride(0), uniforms.data_ptr(), temperature.data_ptr(), n, rows,
-               vocab, _status4(what, status))
+               l_stride, _ints(what, "row_start", row_start, n + 1), drafted_at, p_at, p_stride, uniforms.data_ptr(),
+               temperature.data_ptr(), n, rows, vocab, None if status is None else _ints(what, "status", status, 4))

@@ -23,6 +23,8 @@
 namespace {
 constexpr int PARTS = 8, THREADS = 256, WARPS = THREADS / 32;
 constexpr int MAX_ROWS = 32;
+constexpr int BATCH = 7;                  // 16-byte loads of a thread at a time: a row of up to 57,344 in one go
+constexpr int AHEAD = 8;                  // numbers of a thread asked for together in the second part
 constexpr int KEPT = 8192;                // most exponentials of a CTA's share that are kept (64 KB)
 
 struct VerifyArgs {
@@ -69,6 +71,13 @@ __device__ __forceinline__ double peer_d(const double* p, int rank) {
 }
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// 2^x by the hardware approximation (relative error about 2^-22): a sum of many such terms is off by far less than the
+// 2^-24 that a uniform number of 32 bits can tell apart.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 // (largest value, lowest index among equals)
 __device__ __forceinline__ void better(float& v, int& i, float w, int k) {
@@ -129,56 +138,56 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, 4) veri
         const float* x = p.logits + (long)(r0 + r) * p.logits_stride;
         float top = -INFINITY, sum = 0.0f;
         int index = 0x7fffffff;
-        auto take = [&](const float* v, int n, int first) {          // n logits, of the tokens first, first + 1, ..
-            if (greedy) {
-#pragma unroll
-                for (int i = 0; i < n; ++i) better(top, index, v[i], first + i);
-                return;
-            }
+        auto sums = [&](const auto& v) {
+            constexpr int n = sizeof(v) / sizeof(float);
             float now = top;
 #pragma unroll
             for (int i = 0; i < n; ++i) now = fmaxf(now, v[i]);
             const float ref = now == -INFINITY ? 0.0f : now;
-            sum *= exp2f((top - ref) * scale);
+            sum *= exp2_fast((top - ref) * scale);
 #pragma unroll
-            for (int i = 0; i < n; ++i) sum += exp2f((v[i] - ref) * scale);
+            for (int i = 0; i < n; ++i) sum += exp2_fast((v[i] - ref) * scale);
             top = now;
         };
         // 16 bytes at a time from the first such border on; up to three logits before it and behind the last one alone
         const int head = min((int)((16 - ((uintptr_t)(x + lo) & 15)) & 15) / 4, hi - lo);
         const int vecs = (hi - lo - head) / 4, tail = lo + head + 4 * vecs;
         const float4* body = reinterpret_cast<const float4*>(x + lo + head);
-        for (int i = threadIdx.x; i < vecs; i += 4 * THREADS) {
-            float v[16];
-            int n = 0;
+        for (int i = threadIdx.x; i < vecs; i += BATCH * THREADS) {
+            float v[4 * BATCH];                              // (all asked for before the first is used; -inf weighs nothing)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (i + k * THREADS < vecs) {
-                    const float4 w = body[i + k * THREADS];
-                    v[4 * k] = w.x; v[4 * k + 1] = w.y; v[4 * k + 2] = w.z; v[4 * k + 3] = w.w;
-                    n = k + 1;
-                }
-            if (n == 4 && !greedy) {
-                take(v, 16, 0);
+            for (int k = 0; k < BATCH; ++k) {
+                float4 w = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                if (i + k * THREADS < vecs) w = body[i + k * THREADS];
+                v[4 * k] = w.x; v[4 * k + 1] = w.y; v[4 * k + 2] = w.z; v[4 * k + 3] = w.w;
+            }
+            if (greedy) {
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k)
+                    if (i + k * THREADS < vecs) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) better(top, index, v[4 * k + e], lo + head + 4 * (i + k * THREADS) + e);
+                    }
             } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (k < n) take(v + 4 * k, 4, lo + head + 4 * (i + k * THREADS));
+                sums(v);
             }
         }
         const int lone = threadIdx.x < 4 ? (threadIdx.x < head ? lo + threadIdx.x : hi) : tail + threadIdx.x - 4;
-        if (threadIdx.x < 8 && lone < hi) take(x + lone, 1, lone);
+        if (threadIdx.x < 8 && lone < hi) {
+            const float v[1] = {x[lone]};
+            if (greedy) better(top, index, v[0], lone);
+            else sums(v);
+        }
         // the warp's lanes
+        const float own = top;
+        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(own));
+        if (greedy) {
+            index = (int)__reduce_min_sync(0xffffffffu, (unsigned)(own == top ? index : 0x7fffffff));
+        } else {
+            const float ref = top == -INFINITY ? 0.0f : top;
+            sum *= exp2_fast((own - ref) * scale);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float v = __shfl_xor_sync(0xffffffffu, top, o), w = __shfl_xor_sync(0xffffffffu, sum, o);
-            const int k = __shfl_xor_sync(0xffffffffu, index, o);
-            const float was = top;
-            better(top, index, v, k);
-            if (!greedy) {
-                const float ref = top == -INFINITY ? 0.0f : top;
-                sum = sum * exp2f((was - ref) * scale) + w * exp2f((v - ref) * scale);
-            }
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
         if (lane == 0) {
             s.top[r][warp] = top;
@@ -196,7 +205,7 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, 4) veri
             better(top, index, v, s.index[r][w]);
             if (!greedy) {
                 const float ref = top == -INFINITY ? 0.0f : top;
-                sum = sum * exp2f((was - ref) * scale) + s.sum[r][w] * exp2f((v - ref) * scale);
+                sum = sum * exp2_fast((was - ref) * scale) + s.sum[r][w] * exp2_fast((v - ref) * scale);
             }
         }
         s.top[r][0] = top;
@@ -219,7 +228,7 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, 4) veri
         const float ref = top == -INFINITY ? 0.0f : top;
         if (!greedy) {
 #pragma unroll
-            for (int z = 0; z < PARTS; ++z) sum += peer_f(&s.sum[lane][0], z) * exp2f((part[z] - ref) * scale);
+            for (int z = 0; z < PARTS; ++z) sum += peer_f(&s.sum[lane][0], z) * exp2_fast((part[z] - ref) * scale);
             if (!(fabsf(top) < INFINITY && sum > 0.0f && sum < INFINITY) && rank == 0 && warp == 0)
                 prb_set_status(p.status, PRB_S_LOGITS, r0 + lane, req, 0);
         } else if (!(fabsf(top) < INFINITY) && rank == 0 && warp == 0) {
@@ -274,10 +283,16 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, 4) veri
         const bool keep = each <= KEPT;
         auto raw = [&](int i) -> double { return exp64(((double)x[i] - (double)top) * inverse); };
         double z = 0.0;
-        for (int i = w0 + lane; i < w1; i += 32) {
-            const double e = raw(i);
-            if (keep) kept_e[i - lo] = e;
-            z += e;
+        for (int i0 = w0 + lane; i0 < w1; i0 += 32 * AHEAD) {
+            float v[AHEAD];
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) v[k] = i0 + 32 * k < w1 ? x[i0 + 32 * k] : -INFINITY;
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const double e = exp64(((double)v[k] - (double)top) * inverse);
+                if (keep && i0 + 32 * k < w1) kept_e[i0 + 32 * k - lo] = e;
+                z += e;
+            }
         }
         z = 1.0 / meet(z);
         auto weight = [&](int i, bool less) -> double {
@@ -290,7 +305,18 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, 4) veri
         double whole = 0.0;
         for (int go = 0; go < 2; ++go) {
             double v = 0.0;
-            for (int i = w0 + lane; i < w1; i += 32) v += weight(i, less);
+            if (less && q != nullptr && keep) {
+                for (int i0 = w0 + lane; i0 < w1; i0 += 32 * AHEAD) {
+                    float said[AHEAD];
+#pragma unroll
+                    for (int k = 0; k < AHEAD; ++k) said[k] = i0 + 32 * k < w1 ? q[i0 + 32 * k] : 0.0f;
+#pragma unroll
+                    for (int k = 0; k < AHEAD; ++k)
+                        if (i0 + 32 * k < w1) v += fmax(kept_e[i0 + 32 * k - lo] * z - (double)said[k], 0.0);
+                }
+            } else {
+                for (int i = w0 + lane; i < w1; i += 32) v += weight(i, less);
+            }
             whole = meet(v);
             if (whole > 0.0 || !less) break;
             less = false;                                                 // nothing left: the target's own

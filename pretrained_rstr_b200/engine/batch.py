@@ -99,6 +99,7 @@ class Runtime:
     max_batched_tokens: int = 2048
     max_requests: int = 64
     use_graphs: bool = True            # replay small steps as CUDA graphs
+    cache_bits: Optional[int] = None   # 4: keys and values are cached in 4 bits; None: in ``dtype``
 
     @property
     def serving(self) -> bool:

@@ -70,10 +70,13 @@ class LoadedModel:
 def load_model(folder: str, dtype="bfloat16", device="cuda:0", page_size: int = 64,
                max_batched_tokens: int = 2048, max_requests: int = 64,
                max_tokens: Optional[int] = None, num_pages: Optional[int] = None,
-               share_prefixes: bool = False) -> LoadedModel:
+               share_prefixes: bool = False, cache_bits: Optional[int] = None) -> LoadedModel:
     """``max_tokens``: the most tokens live requests hold at any time, each request's
     count rounded up to whole pages; the page pools are made for that many.  Default:
-    ``max_requests`` requests of full length."""
+    ``max_requests`` requests of full length.  ``cache_bits=4``: keys and values are cached in
+    4 bits (designs whose mixers all are causal attention: GPT-2); None: in ``dtype``."""
+    if cache_bits not in (None, 4):
+        raise ValueError(f"cache_bits must be 4, or None for a cache in the runtime's type; got {cache_bits!r}")
     ops.require_cuda()
     ops.lib()                                   # build / load now, fail loudly here
     ops.set_pdl(SETTINGS.pdl)
@@ -83,7 +86,7 @@ def load_model(folder: str, dtype="bfloat16", device="cuda:0", page_size: int = 
     arch, config = read_config(folder)
     runtime = Runtime(device=device, dtype=dtype, page_size=page_size,
                       max_batched_tokens=max_batched_tokens, max_requests=max_requests,
-                      use_graphs=SETTINGS.graphs)
+                      use_graphs=SETTINGS.graphs, cache_bits=cache_bits)
     store = load_weights(folder, arch.expected_tensors(config), device,
                          strip_prefixes=arch.strip_prefixes, ignorable=arch.ignorable)
     model = arch.build(config, store, runtime)

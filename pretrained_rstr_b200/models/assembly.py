@@ -87,23 +87,27 @@ class Model:
             if e.cache_layer not in writers:
                 raise ValueError(f"run order: layer {e.layer} reads the cache of layer "
                                  f"{e.cache_layer}, which no entry writes")
-        keyed: Dict[Tuple[int, int, object], List[int]] = {}
+        keyed: Dict[Tuple, List[int]] = {}
         for layer in sorted(writers):
             mixer = self.blocks[owner[layer]].mixer
             spec = mixer.kv_spec()
             if spec is not None:
+                wanted = getattr(self.runtime, "cache_bits", None)
+                if spec.bits != wanted:
+                    raise ValueError(f"cache_bits={wanted}: layer {layer}'s mixer ({type(mixer).__name__}) keeps its "
+                                     f"cache in the runtime's type only")
                 keyed.setdefault((spec.kv_heads, spec.head_dim, spec.window,
-                                  2 if spec.values else 1), []).append(layer)
+                                  2 if spec.values else 1, spec.bits), []).append(layer)
             for st in mixer.state_specs():
                 self.state_specs[(layer, st.name)] = st
         for st in self.embedding.state_specs() if hasattr(self.embedding, "state_specs") else ():
             self.state_specs[(-1, st.name)] = st            # (-1: the embedding's own state)
-        for (kv_heads, head_dim, window, pools), layers in sorted(
+        for (kv_heads, head_dim, window, pools, bits), layers in sorted(
                 keyed.items(), key=lambda kv: kv[1][0]):
             name = "full" if window is None else f"window{window}"
             gi = len(self.group_specs)
             self.group_specs.append(GroupSpec(f"{name}.{gi}", tuple(layers), kv_heads, head_dim,
-                                              window, pools))
+                                              window, pools, bits))
             for idx, layer in enumerate(layers):
                 self.layer_group[layer] = (gi, idx)
         for e in self.order:

@@ -157,6 +157,47 @@ class AttentionWork(WorkPlanner):
         return len(items)
 
 
+class Attention4Work(WorkPlanner):
+    """Tiles of a step for the attention over a cache held in 4 bits: a request's tokens in tiles
+    of up to ``128 / group`` (``group``: query heads of a key/value head), those of requests that
+    bring at most ``8 / group`` (decoded and drafted tokens) in a list of their own, whose kernel
+    shares no keys between more rows than that."""
+
+    key = "causal_attention_4bit"
+    counters = ("few", "tiles")
+    launch_steps = {"few": (8, "few_req"), "tiles": (4, "tile_req")}
+
+    def __init__(self, group: int):
+        self.few_most, self.tile_most = max(1, 8 // group), max(1, 128 // group)
+
+    def absorb(self, other: "Attention4Work") -> None:
+        """(mixers with unequal groups share the lists of the larger group: shorter tiles are right for all)"""
+        self.few_most = min(self.few_most, other.few_most)
+        self.tile_most = min(self.tile_most, other.tile_most)
+
+    def arrays(self, t_cap: int, b_cap: int):
+        tiles = t_cap // self.tile_most + b_cap
+        few = min(t_cap, b_cap)
+        return {"few_req": (few, -1), "few_row0": (few, 0), "few_rows": (few, 0),
+                "tile_req": (tiles, -1), "tile_row0": (tiles, 0), "tile_rows": (tiles, 0)}
+
+    def fill(self, arrays: Dict[str, np.ndarray], lengths: Sequence[int]) -> Dict[str, int]:
+        n_few = n_tiles = row = 0
+        for b, n in enumerate(lengths):
+            if n <= self.few_most:
+                arrays["few_req"][n_few], arrays["few_row0"][n_few], arrays["few_rows"][n_few] = b, row, n
+                n_few += 1
+            else:
+                for r in range(0, n, self.tile_most):
+                    arrays["tile_req"][n_tiles], arrays["tile_row0"][n_tiles] = b, row + r
+                    arrays["tile_rows"][n_tiles] = min(self.tile_most, n - r)
+                    n_tiles += 1
+            row += n
+        used = (["few_req", "few_row0", "few_rows"] if n_few else []) + \
+            (["tile_req", "tile_row0", "tile_rows"] if n_tiles else [])
+        return {"few": n_few, "tiles": n_tiles, "_used": used}
+
+
 class CausalAttention(Mixer):
     graph_safe = True
     accepts_lazy_norm = True      # the first matrix product may compute the norm itself
@@ -178,16 +219,24 @@ class CausalAttention(Mixer):
         self.scale, self.window = float(scale), window
         self.runtime = runtime
         self.position = position
+        self.bits = getattr(runtime, "cache_bits", None)
+        if self.bits == 4:
+            ops.cache4_tile_bytes(head_dim, runtime.page_size)      # (refuses sizes it does not take)
+            self.work_plan = Attention4Work(n_head // n_kv_head)
+            return
         self.work_plan = AttentionWork()
         self.work_plan.note_mixer(n_head, window, ops.sm_count() if torch.cuda.is_available() else None)
 
     def kv_spec(self) -> KVSpec:
-        return KVSpec(self.n_kv_head, self.head_dim, self.window)
+        return KVSpec(self.n_kv_head, self.head_dim, self.window, bits=self.bits)
 
     def work_planners(self):
         return [self.work_plan]
 
     def forward(self, ctx, h, x, cache: LayerCache, accumulate: bool = True) -> None:
+        if self.bits == 4:
+            self._forward_4bit(ctx, h, x, cache, accumulate)
+            return
         t = x.shape[0]
         dtype = self.runtime.dtype
         qkv = ctx.scratch("attn_qkv", (ctx.token_capacity, self.qkv.n_out), dtype)[:t]
@@ -213,6 +262,37 @@ class CausalAttention(Mixer):
         # (the step's own keys and values lie beside the queries exactly as the cache got them)
         attend(ctx, o, q, cache, group, self.n_head, self.scale, self.window,
                kv_new=(k, v) if cache.writes else None)
+        self.out.forward(ctx, o, x, resid=x if accumulate else None)
+
+
+    def _forward_4bit(self, ctx, h, x, cache: LayerCache, accumulate: bool) -> None:
+        """The same over a cache held in 4 bits: the step's own keys and values are read back from it
+        too, so that a token sees the same numbers whichever way the work is cut."""
+        t = x.shape[0]
+        dtype = self.runtime.dtype
+        qkv = ctx.scratch("attn_qkv", (ctx.token_capacity, self.qkv.n_out), dtype)[:t]
+        group = ctx.groups[cache.group]
+        self.qkv.forward(ctx, h, qkv)
+        q = qkv[:, :self.q_width]
+        k = qkv[:, self.q_width:self.q_width + self.kv_width]
+        v = qkv[:, self.q_width + self.kv_width:]
+        if self.position is not None:
+            self.position.rotate(ctx, q, k)
+        if cache.writes:
+            ops.kv_append_4bit(cache.k, cache.v, k, v, group.slots, t, self.head_dim, group.page_size, ctx.status)
+        o = ctx.scratch("attn_out", (ctx.token_capacity, self.q_width), dtype)[:t]
+        work = ctx.work[Attention4Work.key]
+        for name, most in (("few", work.planner.few_most if ctx.max_q_len > 1 else 1), ("tile", work.planner.tile_most)):
+            counter = "few" if name == "few" else "tiles"
+            n = work.host_counts[counter]
+            if n == 0:
+                continue
+            if n is None:                       # (a step that runs as a graph: the count is on the device)
+                n = work.launch.get(counter, work.caps[name + "_req"])
+            lists = [work.arrays[f"{name}_{part}"][:n] for part in ("req", "row0", "rows")]
+            ops.attention_4bit(o, q, cache.k, cache.v, group.block_table, ctx.positions, *lists, most, self.n_head,
+                               self.head_dim, group.page_size, self.scale, self.window, ctx.max_context, ctx.status,
+                               tile_count=work.counts[counter])
         self.out.forward(ctx, o, x, resid=x if accumulate else None)
 
 

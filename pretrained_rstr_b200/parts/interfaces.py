@@ -27,6 +27,7 @@ class KVSpec:
     head_dim: int
     window: Optional[int] = None      # None: all keys; w: only the last w
     values: bool = True               # False: one row per token serves as key and value
+    bits: Optional[int] = None        # 4: pages held in 4 bits (``ops.kv_append_4bit``); None: the runtime's type
 
 
 @dataclass(frozen=True)
@@ -40,7 +41,8 @@ class StateSpec:
 @dataclass
 class LayerCache:
     """What a block hands to its mixer: the pages of the cache layer it attends over
-    (``k``/``v``: [pages, kv_heads, page_size, head_dim]; ``group`` indexes
+    (``k``/``v``: [pages, kv_heads, page_size, head_dim], or uint8 [pages, kv_heads, bytes of a tile]
+    where the group holds 4 bits; ``group`` indexes
     ``ctx.groups``), whether this run entry writes them, and its state tensors."""
     group: int = -1
     k: Optional[torch.Tensor] = None

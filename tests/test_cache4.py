@@ -79,6 +79,7 @@ def ops(monkeypatch):
     def launched(*_a, **_k):
         raise AssertionError("a refused call reached the library")
     monkeypatch.setattr(module, "lib", launched)
+    monkeypatch.setattr(module, "_LIB", None)
     return module
 
 
