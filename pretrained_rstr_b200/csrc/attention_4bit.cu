@@ -1,11 +1,21 @@
 // Causal attention over a cache held in 4 bits: the launch, and the bfloat16 form of the kernel in attention_4bit.cuh.
 #include "attention_4bit.cuh"
 
-// (attention_4bit_f32.cu, attention_4bit_rows.cu)
+// (attention_4bit_tile.cu, attention_4bit_f32.cu, attention_4bit_rows.cu)
+bool prb_attention_4bit_tile_takes(int head_dim, int page_size, int window, const void* q, long q_stride, const void* out,
+                                   long out_stride);
+int prb_attention_4bit_tile(void* out, long out_stride, const void* q, long q_stride, const uint8_t* k_tiles,
+                            const uint8_t* v_tiles, const int* block_table, const int* positions, const int* tile_req,
+                            const int* tile_row0, const int* tile_rows, const int* tile_count, int n_tiles, long rows,
+                            int n_tokens, int n_requests, int kv_heads, int hpg, int head_dim, int page_size, int max_pages,
+                            int num_pages, float scale, int max_context, int parts, int* status, cudaStream_t stream);
 int prb_attention_4bit_f32(const attn4::Args& p, long rows, int max_context, int parts, cudaStream_t stream);
 int prb_attention_4bit_rows(const attn4::Args& p, long rows, int max_context, int parts, cudaStream_t stream);
 
 namespace {
+// More rows than this go to the tensor-memory kernel where it takes the call.
+constexpr long TILE_ROWS = 32;
+
 // up to 4 rows a tile, or 8
 template <int NG> int by(const attn4::Args& p, long rows, int max_context, int parts, cudaStream_t stream) {
     return rows <= 4 ? attn4::launch_by<NG, 1, 1, __nv_bfloat16>(p, rows, max_context, parts, stream)
@@ -52,6 +62,10 @@ PRB_API int prb_attention_4bit(void* out, long out_stride, const void* q, long q
     p.magic = 0x43004300u;
     const long rows = (long)tile_most * hpg;
     if (dtype == PRB_F32) return prb_attention_4bit_f32(p, rows, max_context, parts, stream);
+    if (rows > TILE_ROWS && prb_attention_4bit_tile_takes(head_dim, page_size, window, q, q_stride, out, out_stride))
+        return prb_attention_4bit_tile(out, out_stride, q, q_stride, p.k_tiles, p.v_tiles, block_table, positions, tile_req,
+                                       tile_row0, tile_rows, tile_count, n_tiles, rows, n_tokens, n_requests, kv_heads, hpg,
+                                       head_dim, page_size, max_pages, num_pages, scale, max_context, parts, status, stream);
     return rows <= 8 ? launch_few(p, rows, max_context, parts, stream)
                      : prb_attention_4bit_rows(p, rows, max_context, parts, stream);
 }

@@ -716,7 +716,7 @@ attention_4bit_kernel(const Args p) {
         if (ch < head_dim) {
             const int at = first + row, tk = at / p.hpg, h = hk * p.hpg + at - tk * p.hpg;
             reinterpret_cast<T*>(p.out)[(long)(row0 + tk) * p.out_stride + (long)h * head_dim + ch] =
-                prb_from_float<T>(sum > 0.0f ? x / sum : 0.0f);
+                prb_from_float<T>(sum > 0.0f || sum != sum ? x / sum : 0.0f);      // (a NaN goes on)
         }
     }
     if (p.parts > 1) cluster_sync_all();                       // nobody leaves while its state may be read

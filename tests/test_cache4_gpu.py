@@ -170,6 +170,13 @@ CASES = [
     ([5000], [1], 2, 1, 64, 64, None),
     ([3000], [2], 4, 1, 128, 16, 2500),
     ([10], [1], 40, 1, 64, 64, None),
+    # portions of prompts that go to the tensor-memory kernel
+    ([0], [33], 2, 2, 64, 64, None),
+    ([130, 5, 0], [70, 200, 64], 4, 4, 64, 64, None),
+    ([300, 64], [40, 64], 8, 2, 128, 64, None),
+    ([1000], [128], 1, 1, 64, 128, None),
+    ([700, 63], [65, 129], 2, 1, 128, 192, None),
+    ([0], [50], 40, 1, 64, 64, None),
 ]
 
 
@@ -179,7 +186,7 @@ CASES = [
 def test_attention_against_64_bits(case, parts, dtype):
     ops = _ops()
     held, new, heads, kv, d, page, window = CASES[case]
-    if parts in (1, 3) and case not in (1, 3, 5, 13):
+    if parts in (1, 3) and case not in (1, 3, 5, 13, 17, 19):
         pytest.skip("one or two long cases are enough for a forced number of parts")
     g = torch.Generator().manual_seed(case)
     total = [a + n for a, n in zip(held, new)]
@@ -216,6 +223,39 @@ def test_attention_against_64_bits(case, parts, dtype):
     again = torch.zeros_like(out)
     ops.attention_4bit(again, qd[:, :heads * d], *args, parts=parts)
     assert torch.equal(again[:-2], out[:-2])                              # the same bits every time
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv,d,page,new", [(2, 2, 64, 64, 80), (4, 1, 128, 64, 30), (2, 1, 96, 32, 40), (1, 1, 64, 64, 3)])
+@pytest.mark.parametrize("parts", [0, 1, 4])
+def test_a_token_that_is_no_number_reaches_those_that_see_it(heads, kv, d, page, new, dtype, parts):
+    """A NaN among a token's keys makes that token's and all later results NaN in the heads that share it; one among its
+    values in the channels of its group; what comes before it in the same tile stays what it was."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(new)
+    held, bad_k, bad_v = 70, 70 + new - 2, 70 + new // 2
+    total = held + new
+    pages = -(-total // page)
+    k, v = (torch.randn(pages * page, kv, d, generator=g) for _ in range(2))
+    clean = [plain.pack(*plain.quantize(x.view(pages, page, kv, d).transpose(1, 2))) for x in (k, v)]
+    k[bad_k, 0, 3], v[bad_v, kv - 1, d - 1] = math.nan, math.inf
+    dirty = [plain.pack(*plain.quantize(x.view(pages, page, kv, d).transpose(1, 2))) for x in (k, v)]
+    q = torch.randn(new, heads * d, generator=g).to(dtype).to(CUDA)
+    tiles = plain.tiles_of([new], max(1, 128 * kv // heads))
+    out = []
+    for kt, vt in (clean, dirty):
+        o, status = torch.zeros(new, heads * d, dtype=dtype, device=CUDA), _status()
+        ops.attention_4bit(o, q, kt.to(CUDA), vt.to(CUDA), _ints([list(range(pages))]), _ints(list(range(held, total))),
+                           *(_ints(list(x)) for x in zip(*tiles)), min(new, max(1, 128 * kv // heads)), heads, d, page, 0.3,
+                           None, total, status, parts=parts)
+        assert status.tolist() == [0] * 4
+        out.append(o.float().cpu().view(new, heads, d))
+    nan = torch.zeros(new, heads, d, dtype=torch.bool)
+    group = heads // kv
+    nan[bad_k - held:, :group] = True
+    nan[bad_v - held:, heads - group:, (d - 1) // 32 * 32:] = True
+    assert torch.equal(torch.isnan(out[1]), nan)
+    assert torch.equal(out[0][~nan], out[1][~nan])
 
 
 # --------------------------------------------------------------------------------------- tables
