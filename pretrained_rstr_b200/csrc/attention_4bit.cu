@@ -13,7 +13,9 @@ int prb_attention_4bit_f32(const attn4::Args& p, long rows, int max_context, int
 int prb_attention_4bit_rows(const attn4::Args& p, long rows, int max_context, int parts, cudaStream_t stream);
 
 namespace {
-// More rows than this go to the tensor-memory kernel where it takes the call.
+// More rows than this go to the tensor-memory kernel where it takes the call: 33 tokens at 300 of 12 heads of 64 20.8 us by
+// the other one, 13.1 by that; 8 x 33 at 1,000 28.0 and 25.5; 16 x 64 at 500 of 16 heads 48.9 and 25.3; 20 x 12 tokens of
+// 4 heads a key/value head of 128 59.5 and 46.6.
 constexpr long TILE_ROWS = 32;
 
 // up to 4 rows a tile, or 8

@@ -543,8 +543,16 @@ attention_4bit_kernel(const Args p) {
                 for (int z = 0; z < QN; ++z) {
                     uint32_t b0[PIECES], b1[PIECES];
                     as_operand<EN, PIECES>(s[c][z], lane, b0, b1);
+                    if (EXACT) {
+                        float part[4];
+                        mma0(part, a0, 0u, a1, 0u, b0[PIECES - 1], b1[PIECES - 1]);
 #pragma unroll
-                    for (int k = PIECES - 1; k >= 0; --k) mma(mid[z], a0, 0u, a1, 0u, b0[k], b1[k]);
+                        for (int k = PIECES - 2; k >= 0; --k) mma(part, a0, 0u, a1, 0u, b0[k], b1[k]);
+#pragma unroll
+                        for (int e = 0; e < EN; ++e) mid[z][e] += part[e];
+                    } else {
+                        mma(mid[z], a0, 0u, a1, 0u, b0[0], b1[0]);
+                    }
                 }
             } else {
                 // A masked key's middle may be anything, NaN too, which a product would spread over all rows.
@@ -592,10 +600,27 @@ attention_4bit_kernel(const Args p) {
                     }
                     uint32_t b0[PIECES], b1[PIECES];
                     as_operand<EN, PIECES>(x, lane, b0, b1);
+                    if (EXACT) {
+                        // The matrix units cut what a sum in 32 bits does not hold instead of rounding it, and thousands
+                        // of keys make that a drift (1.7e-6 at contexts of some 10,000): 16 keys at a time there, the
+                        // rest in sums that round.
+                        float part[2][4];
+                        mma0(part[0], a[0][0], a[1][0], a[0][1], a[1][1], b0[PIECES - 1], b1[PIECES - 1]);
+                        mma0(part[1], a[2][0], a[3][0], a[2][1], a[3][1], b0[PIECES - 1], b1[PIECES - 1]);
 #pragma unroll
-                    for (int k = PIECES - 1; k >= 0; --k) {
-                        mma(o[z][g][0], a[0][0], a[1][0], a[0][1], a[1][1], b0[k], b1[k]);
-                        mma(o[z][g][1], a[2][0], a[3][0], a[2][1], a[3][1], b0[k], b1[k]);
+                        for (int k = PIECES - 2; k >= 0; --k) {
+                            mma(part[0], a[0][0], a[1][0], a[0][1], a[1][1], b0[k], b1[k]);
+                            mma(part[1], a[2][0], a[3][0], a[2][1], a[3][1], b0[k], b1[k]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if ((e & 1) >= EN) continue;
+                            o[z][g][0][e] += part[0][e];
+                            o[z][g][1][e] += part[1][e];
+                        }
+                    } else {
+                        mma(o[z][g][0], a[0][0], a[1][0], a[0][1], a[1][1], b0[0], b1[0]);
+                        mma(o[z][g][1], a[2][0], a[3][0], a[2][1], a[3][1], b0[0], b1[0]);
                     }
                 }
             }
@@ -753,7 +778,11 @@ template <int NG, int QN, int EN, typename T> int launch_by(Args p, long rows, i
     const long subs = (rows + most - 1) / most, units = (long)p.n_tiles * p.kv_heads * subs;
     if (units > 0x7fffffffL / MAX_PARTS) return PRB_E_SIZE;
     p.subs = (int)subs;
-    p.warps = MAX_WARPS;
+    // Four warps a CTA; two once the units alone fill the SMs with four such CTAs each: a warp then has twice the stages to
+    // one set-up and half as many states to merge.  64 tokens at 1,000 of 12 heads (768 units) 27.9 us with four, 23.3 with
+    // two; at 300 of 16 heads (1,024) 15.6 and 13.6; 24 x 5 tokens of 16 heads (384) 14.4 and 19.7; float32 texts (more
+    // instructions a stage) 30.9 and 39.8.
+    p.warps = QN == 1 && sizeof(T) == 2 && units > 4L * prb_sm_count() ? 2 : MAX_WARPS;
     // Parts of a unit's keys: as many as give every SM about four CTAs, each with a stage a warp at least.  (The longest
     // request's: max_context, or what a window and the tile's own tokens span.)
     const int reach = p.window > 0 ? min((long)max_context, (long)p.window + p.tile_most + sk) : max_context;

@@ -7,7 +7,7 @@
 //          bfloat16 is 16) into a ring of raw stages;
 //   1      allocates tensor memory; one thread issues tcgen05.mma: S = Q K^T (128 x 64), O += P V;
 //   2-9    softmax: two threads a row, each 32 of a block's 64 scores and half of the output's channels;
-//   10-13  turn codes into operands in the swizzled layout, once for all 128 rows.
+//   10-17  turn codes into operands in the swizzled layout, once for all 128 rows.
 // Values become bfloat16 (2^-8 of a value, as a bfloat16 cache would hold it, on top of the cache's own rounding).  Keys
 // become the sum of two bfloat16 numbers and take two products: a key's rounding moves a score by the product of the
 // query's and the key's lengths times it, which at ordinary scores is several times what P's rounding costs, and the tensor
@@ -19,6 +19,8 @@
 //
 // Every wait is bounded: where one gives up the status word says so, nothing more is stored, copies in flight are waited
 // for, tensor memory is freed.
+#include <type_traits>
+
 #include "cache4.cuh"
 #include "tcgen05.cuh"
 
@@ -26,8 +28,8 @@ namespace {
 using namespace tc5;
 
 constexpr int QT = 128, KB = 64;
-constexpr int SOFTMAX = 8, DEQUANT = 4, WARPS = 2 + SOFTMAX + DEQUANT, THREADS = WARPS * 32;
-constexpr int RAW_STAGES = 2, STAGES = 2, MAX_PARTS = 4;
+constexpr int SOFTMAX = 8, DEQUANT = 8, WARPS = 2 + SOFTMAX + DEQUANT, THREADS = WARPS * 32;
+constexpr int RAW_STAGES = 3, STAGES = 2, MAX_PARTS = 4;
 constexpr int P_BYTES = QT * KB * 2;
 constexpr float RESCALE_STEP = 8.0f;         // a row's reference maximum moves only by more than this (log2 units)
 
@@ -59,6 +61,7 @@ struct Params {
     int n_tokens, n_requests, n_tiles, subs, parts;
     int kv_heads, hpg, page_size, max_pages, num_pages, tile_bytes;
     float scale;
+    uint32_t magic;                         // 0x43004300: a constant that the compiler keeps in a register
     int* status;
 };
 
@@ -70,15 +73,23 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+// 32 lanes x 16 consecutive 32-bit columns, to and from tensor memory.
+__device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -115,9 +126,11 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
     uint64_t* bars = reinterpret_cast<uint64_t*>(raw + RAW_STAGES * 2 * RAW);
     uint64_t* raw_full = bars;                   // [RAW_STAGES] copies -> dequant
     uint64_t* raw_empty = raw_full + RAW_STAGES; // dequant -> copies
-    uint64_t* kv_full = raw_empty + RAW_STAGES;  // [STAGES] dequant -> MMA
-    uint64_t* kv_empty = kv_full + STAGES;       // MMA -> dequant
-    uint64_t* s_full = kv_empty + STAGES;        // [2] scores ready
+    uint64_t* k_full = raw_empty + RAW_STAGES;   // [STAGES] dequant -> MMA
+    uint64_t* k_empty = k_full + STAGES;         // MMA -> dequant: a block's keys are free before its softmax begins
+    uint64_t* v_full = k_empty + STAGES;
+    uint64_t* v_empty = v_full + STAGES;
+    uint64_t* s_full = v_empty + STAGES;         // [2] scores ready
     uint64_t* q_full = s_full + 2;
     uint64_t* p_full = q_full + 1;
     uint64_t* o_full = p_full + 1;
@@ -161,8 +174,10 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
             mbar_init(smem_u32(&raw_empty[s]), DEQUANT);
         }
         for (int s = 0; s < STAGES; ++s) {
-            mbar_init(smem_u32(&kv_full[s]), DEQUANT);
-            mbar_init(smem_u32(&kv_empty[s]), 1);
+            mbar_init(smem_u32(&k_full[s]), DEQUANT);
+            mbar_init(smem_u32(&k_empty[s]), 1);
+            mbar_init(smem_u32(&v_full[s]), DEQUANT);
+            mbar_init(smem_u32(&v_empty[s]), 1);
         }
         mbar_init(smem_u32(&s_full[0]), 1);
         mbar_init(smem_u32(&s_full[1]), 1);
@@ -255,24 +270,26 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
                                       part > 0 || a > 0 || kk > 0 ? 1u : 0u);
                     }
                 umma_commit(smem_u32(&s_full[j & 1]));
+                umma_commit(smem_u32(&k_empty[j % STAGES]));
             }
             __syncwarp();
         };
         if (n_blocks > 0) {
             ok = mbar_wait_warp(smem_u32(q_full), 0, failed);
-            if (ok) ok = mbar_wait_warp(smem_u32(&kv_full[0]), 0, failed);
+            if (ok) ok = mbar_wait_warp(smem_u32(&k_full[0]), 0, failed);
             if (ok) {
                 tcgen05_fence_after();
                 issue_scores(0);
             }
             for (int j = 0; j < n_blocks && ok; ++j) {
                 if (j + 1 < n_blocks) {
-                    ok = mbar_wait_warp(smem_u32(&kv_full[(j + 1) % STAGES]), ((j + 1) / STAGES) & 1, failed);
+                    ok = mbar_wait_warp(smem_u32(&k_full[(j + 1) % STAGES]), ((j + 1) / STAGES) & 1, failed);
                     if (!ok) break;
                     tcgen05_fence_after();
                     issue_scores(j + 1);
                 }
-                ok = mbar_wait_warp(smem_u32(p_full), j & 1, failed);
+                ok = mbar_wait_warp(smem_u32(&v_full[j % STAGES]), (j / STAGES) & 1, failed);
+                if (ok) ok = mbar_wait_warp(smem_u32(p_full), j & 1, failed);
                 if (!ok) break;
                 tcgen05_fence_after();
                 const uint32_t v_addr = smem_u32(ring + (size_t)(j % STAGES) * STAGE) + 2 * ND * TILE;
@@ -284,7 +301,7 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
                             umma_bf16(tmem_base + O_COL + a * 64, p_desc + (uint64_t)(kk * 2),
                                       make_smem_desc(v_addr + a * TILE + kk * 2048), idesc_o, j > 0 || kk > 0 ? 1u : 0u);
                     umma_commit(smem_u32(o_full));
-                    umma_commit(smem_u32(&kv_empty[j % STAGES]));
+                    umma_commit(smem_u32(&v_empty[j % STAGES]));
                 }
                 __syncwarp();
             }
@@ -306,7 +323,9 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
                 const int ci = half * 4 * ND + c;
                 uint4 w = make_uint4(0u, 0u, 0u, 0u);
                 if (row_ok) w = *reinterpret_cast<const uint4*>(src + ci * 8);
-                st_shared_v4(smem_u32(q_s) + (ci >> 3) * QT * 128 + r * 128 + (((ci & 7) ^ (r & 7)) << 4), w.x, w.y, w.z, w.w);
+                st_shared_v4(smem_u32(q_s) + (ci >> 3) * QT * 128 + r * 128 + (((ci & 7) ^ (r & 7)) << 4),
+                             __byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632),
+                             __byte_perm(w.y, w.w, 0x5410), __byte_perm(w.y, w.w, 0x7632));
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -317,25 +336,32 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
             // After a wait gave up the warp still walks every block, without waiting or touching tensor memory, so that
             // the barriers of its thread pairs stay matched.
             if (ok) ok = mbar_wait_warp(smem_u32(&s_full[j & 1]), (j >> 1) & 1, failed);
-            uint32_t sr[HC];
-            if (ok) {
-                tcgen05_fence_after();
-                tmem_ld_32x32(lane_addr + (uint32_t)((j & 1) * KB + half * HC), sr);
-            } else {
-#pragma unroll
-                for (int c = 0; c < HC; ++c) sr[c] = 0u;
-            }
             const int key0 = (blk_lo + j) * KB + half * HC;
-            if (key0 + HC - 1 > qpos) {
+            const bool diagonal = key0 + HC - 1 > qpos;
+            const uint32_t s_addr = lane_addr + (uint32_t)((j & 1) * KB + half * HC);
+            // 16 scores at a time, read twice (for the maximum, for the exponentials): registers for two CTAs an SM
+            auto scores = [&](int c0, uint32_t (&sr)[16]) {
+                if (ok) {
+                    tmem_ld_16(s_addr + (uint32_t)c0, sr);
+                } else {
 #pragma unroll
-                for (int c = 0; c < HC; ++c)
-                    if (key0 + c > qpos) sr[c] = 0xff800000u;              // -inf
-            }
+                    for (int c = 0; c < 16; ++c) sr[c] = 0u;
+                }
+                if (diagonal) {
+#pragma unroll
+                    for (int c = 0; c < 16; ++c)
+                        if (key0 + c0 + c > qpos) sr[c] = 0xff800000u;     // -inf
+                }
+            };
+            if (ok) tcgen05_fence_after();
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < HC; c += 4)
+            for (int c0 = 0; c0 < HC; c0 += 16) {
+                uint32_t sr[16];
+                scores(c0, sr);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mx4[e] = fmaxf(mx4[e], __uint_as_float(sr[c + e]));
+                for (int c = 0; c < 16; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], __uint_as_float(sr[c]));
+            }
             const float mx_own = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
             xmax[((j & 1) * 2 + half) * QT + r] = mx_own;
             asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");
@@ -348,17 +374,6 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
             const float corr = rescale ? exp2_fast(m_run - m_new) : 1.0f;
             m_run = m_new;
             const float neg_m = m_new == -INFINITY ? 0.0f : -m_new;
-            uint32_t pk[HC / 2];
-            float rs0 = 0.0f, rs1 = 0.0f;
-#pragma unroll
-            for (int c = 0; c < HC; c += 2) {
-                const float p0 = exp2_fast(fmaf(__uint_as_float(sr[c]), sl2, neg_m));
-                const float p1 = exp2_fast(fmaf(__uint_as_float(sr[c + 1]), sl2, neg_m));
-                rs0 += p0;
-                rs1 += p1;
-                pk[c >> 1] = pack2(p0, p1);
-            }
-            l_run = l_run * corr + (rs0 + rs1);
             // the product of the block before has retired: P is free and the results may be touched
             if (ok && j >= 1) {
                 ok = mbar_wait_warp(smem_u32(o_full), (j - 1) & 1, failed);
@@ -366,18 +381,33 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
             }
             if (ok && __any_sync(0xffffffffu, rescale)) {
 #pragma unroll
-                for (int a = 0; a < ND; ++a) {
-                    uint32_t ob[32];
-                    tmem_ld_32x32(lane_addr + O_COL + (uint32_t)((half * ND + a) * 32), ob);
+                for (int c0 = 0; c0 < 32 * ND; c0 += 16) {
+                    uint32_t ob[16];
+                    tmem_ld_16(lane_addr + O_COL + (uint32_t)(half * ND * 32 + c0), ob);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) ob[i] = __float_as_uint(__uint_as_float(ob[i]) * corr);
-                    tmem_st_32x32(lane_addr + O_COL + (uint32_t)((half * ND + a) * 32), ob);
+                    for (int i = 0; i < 16; ++i) ob[i] = __float_as_uint(__uint_as_float(ob[i]) * corr);
+                    tmem_st_16(lane_addr + O_COL + (uint32_t)(half * ND * 32 + c0), ob);
                 }
             }
+            float rs0 = 0.0f, rs1 = 0.0f;
 #pragma unroll
-            for (int c = 0; c < HC / 8; ++c)
-                st_shared_v4(smem_u32(p_s) + r * 128 + (((half * 4 + c) ^ (r & 7)) << 4), pk[4 * c], pk[4 * c + 1],
-                             pk[4 * c + 2], pk[4 * c + 3]);
+            for (int c0 = 0; c0 < HC; c0 += 16) {
+                uint32_t sr[16], pk[8];
+                scores(c0, sr);
+#pragma unroll
+                for (int c = 0; c < 16; c += 2) {
+                    const float p0 = exp2_fast(fmaf(__uint_as_float(sr[c]), sl2, neg_m));
+                    const float p1 = exp2_fast(fmaf(__uint_as_float(sr[c + 1]), sl2, neg_m));
+                    rs0 += p0;
+                    rs1 += p1;
+                    pk[c >> 1] = pack2(p0, p1);
+                }
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    st_shared_v4(smem_u32(p_s) + r * 128 + (((half * 4 + c0 / 8 + c) ^ (r & 7)) << 4), pk[4 * c], pk[4 * c + 1],
+                                 pk[4 * c + 2], pk[4 * c + 3]);
+            }
+            l_run = l_run * corr + (rs0 + rs1);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tcgen05_fence_before();
             __syncwarp();
@@ -394,61 +424,82 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
         // ------------------------------------------------- codes to operands
         const int t = (warp - 2 - SOFTMAX) * 32 + lane;
         const int key8 = lane & 7, w = lane >> 3;                 // a key of 8, a word of a group's 4: no bank twice
-        for (int j = 0; j < n_blocks; ++j) {
+        // One block's keys (KIND 0) or values: 8 keys x a group's 4 words at a time, 8 (keys) x NG of them, an eighth for each
+        // warp; all words are asked for before the first is used.
+        auto convert = [&](int j, auto kind_t) -> bool {
+            constexpr int KIND = decltype(kind_t)::value;
             const int rs = j % RAW_STAGES, st = j % STAGES, key0 = (blk_lo + j) * KB;
-            ok = mbar_wait_warp(smem_u32(&raw_full[rs]), (j / RAW_STAGES) & 1, failed);
-            if (ok) ok = mbar_wait_warp(smem_u32(&kv_empty[st]), ((j / STAGES) & 1) ^ 1, failed);
-            if (!ok) {
+            bool fine = KIND == 0 ? mbar_wait_warp(smem_u32(&raw_full[rs]), (j / RAW_STAGES) & 1, failed) : true;
+            if (fine) fine = mbar_wait_warp(smem_u32(KIND == 0 ? &k_empty[st] : &v_empty[st]), ((j / STAGES) & 1) ^ 1, failed);
+            if (!fine) {
                 if (lane == 0) prb_set_status(p.status, PRB_S_WAIT_TIMEOUT, 46, blockIdx.x, j);
-                break;
+                return false;
             }
-            const uint8_t* src = raw + rs * 2 * RAW;
-            const uint32_t stage = smem_u32(ring + (size_t)st * STAGE);
-            // 8 keys x a group's 4 words at a time: 8 (keys) x NG of them, a quarter for each warp
+            const uint8_t* src = raw + rs * 2 * RAW + KIND * RAW;
+            const uint32_t stage = smem_u32(ring + (size_t)st * STAGE) + KIND * 2 * ND * TILE;
+            constexpr int TASKS = 8 * NG / DEQUANT;
+            uint32_t word[TASKS], pair[TASKS];
 #pragma unroll
-            for (int kind = 0; kind < 2; ++kind)
+            for (int i = 0; i < TASKS; ++i) {
+                const int task = (t >> 5) + i * DEQUANT, g = task >> 3, key = (task & 7) * 8 + key8;
+                word[i] = *reinterpret_cast<const uint32_t*>(src + g * KB * 16 + key * 16 + w * 4);
+                pair[i] = *reinterpret_cast<const uint32_t*>(src + KB * (D / 2) + (key * NG + g) * 4);
+            }
+            // (channels i and i + 4 of a word's 8 lie together, as one shift and one mask take them from it: the queries are
+            // laid out alike, and the results' channels are put right when they are stored)
 #pragma unroll
-                for (int i = 0; i < 2 * NG; ++i) {
-                    const int task = (t >> 5) + i * DEQUANT, g = task >> 3, key = (task & 7) * 8 + key8;
-                    const uint32_t word = *reinterpret_cast<const uint32_t*>(src + kind * RAW + g * KB * 16 + key * 16 + w * 4);
-                    const uint32_t pair =
-                        *reinterpret_cast<const uint32_t*>(src + kind * RAW + KB * (D / 2) + (key * NG + g) * 4);
-                    float step = __uint_as_float(pair << 16), middle = __uint_as_float(pair & 0xffff0000u);
-                    if (kind == 1 && key0 + key > pos_lo) {
+            for (int i = 0; i < TASKS; ++i) {
+                const int task = (t >> 5) + i * DEQUANT, g = task >> 3, key = (task & 7) * 8 + key8;
+                const int chunk = (g & 1) * 4 + w;                        // of the row's 8 pieces of 8 channels
+                const uint32_t at = stage + (g >> 1) * TILE + key * 128 + ((chunk ^ (key & 7)) << 4);
+                uint32_t hi[4];
+                if (KIND == 1) {
+                    if (key0 + KB - 1 > pos_lo && key0 + key > pos_lo) {
                         // not seen by all rows: by none (stale), or by some, and then it may be no number
-                        const bool number = fabsf(step) < INFINITY && fabsf(middle) < INFINITY;
+                        const bool number = (pair[i] & 0x7f80u) != 0x7f80u && (pair[i] & 0x7f800000u) != 0x7f800000u;
                         if (!number && key0 + key <= pos_hi && w == 0) atomicMin(&poison[g], key0 + key);
-                        if (!number || key0 + key > pos_hi) step = middle = 0.0f;
+                        if (!number || key0 + key > pos_hi) pair[i] = 0u;
                     }
-                    const float base = fmaf(step, -136.0f, middle);           // (the codes come as 128 + c)
-                    float x[8];
+                    // middle + step * (c - 8), rounded once
+                    const uint32_t step = __byte_perm(pair[i], 0u, 0x1010), middle = __byte_perm(pair[i], 0u, 0x3232);
+                    const __nv_bfloat162 off = __floats2bfloat162_rn(136.0f, 136.0f);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const uint32_t u = ((word >> (4 * e)) & 0x000f000fu) | 0x43004300u;
-                        x[e] = fmaf(step, __uint_as_float(u << 16), base);
-                        x[e + 4] = fmaf(step, __uint_as_float(u & 0xffff0000u), base);
+                        const uint32_t u = ((word[i] >> (4 * e)) & 0x000f000fu) | p.magic;
+                        const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&step),
+                                                         __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), off),
+                                                         *reinterpret_cast<const __nv_bfloat162*>(&middle));
+                        hi[e] = *reinterpret_cast<const uint32_t*>(&v);
                     }
-                    uint32_t hi[4];
+                    st_shared_v4(at, hi[0], hi[1], hi[2], hi[3]);
+                } else {
+                    const float step = __uint_as_float(pair[i] << 16);
+                    const float base = fmaf(step, -136.0f, __uint_as_float(pair[i] & 0xffff0000u));   // (codes come as 128 + c)
+                    uint32_t lo[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) hi[e] = pack2(x[2 * e], x[2 * e + 1]);
-                    const int chunk = (g & 1) * 4 + w;                        // of the row's 8 pieces of 8 channels
-                    const uint32_t at = (g >> 1) * TILE + key * 128 + ((chunk ^ (key & 7)) << 4);
-                    st_shared_v4(stage + (kind ? 2 * ND * TILE : 0) + at, hi[0], hi[1], hi[2], hi[3]);
-                    if (kind == 0) {
-                        uint32_t lo[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            lo[e] = pack2(x[2 * e] - __uint_as_float(hi[e] << 16),
-                                          x[2 * e + 1] - __uint_as_float(hi[e] & 0xffff0000u));
-                        st_shared_v4(stage + ND * TILE + at, lo[0], lo[1], lo[2], lo[3]);
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t u = ((word[i] >> (4 * e)) & 0x000f000fu) | p.magic;
+                        const float x0 = fmaf(step, __uint_as_float(u << 16), base);
+                        const float x1 = fmaf(step, __uint_as_float(u & 0xffff0000u), base);
+                        hi[e] = pack2(x0, x1);
+                        lo[e] = pack2(x0 - __uint_as_float(hi[e] << 16), x1 - __uint_as_float(hi[e] & 0xffff0000u));
                     }
+                    st_shared_v4(at, hi[0], hi[1], hi[2], hi[3]);
+                    st_shared_v4(at + ND * TILE, lo[0], lo[1], lo[2], lo[3]);
                 }
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(smem_u32(&raw_empty[rs]));
-                mbar_arrive(smem_u32(&kv_full[st]));
+                if (KIND == 1) mbar_arrive(smem_u32(&raw_empty[rs]));
+                mbar_arrive(smem_u32(KIND == 0 ? &k_full[st] : &v_full[st]));
             }
+            return true;
+        };
+        // (a block's values after the next one's keys, which are wanted first)
+        for (int j = 0; j <= n_blocks && ok; ++j) {
+            if (j < n_blocks) ok = convert(j, std::integral_constant<int, 0>());
+            if (ok && j > 0) ok = convert(j - 1, std::integral_constant<int, 1>());
         }
     }
 
@@ -462,27 +513,32 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
     constexpr int HD = D / 2;
     const int row = first + min(r, rows - 1), tk = row / p.hpg, qpos = pos0 + tk;
     __nv_bfloat16* dst = p.out + (long)(row0 + tk) * p.out_stride + (long)(hk * p.hpg + row - tk * p.hpg) * D;
-    auto store8 = [&](int ch, const float (&x)[8], float inv) {
+    // 8 channels from ch on, x in the operands' order (0, 4, 1, 5, 2, 6, 3, 7)
+    auto store8 = [&](int ch, const float (&x)[8], float inv, bool bad) {
+        const float nan = __int_as_float(0x7fc00000);
         float y[8];
-        const bool bad = qpos >= poison[ch >> 5];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = bad ? __int_as_float(0x7fc00000) : x[i] * inv;
+        for (int i = 0; i < 4; ++i) {
+            y[i] = bad ? nan : x[2 * i] * inv;
+            y[i + 4] = bad ? nan : x[2 * i + 1] * inv;
+        }
         *reinterpret_cast<uint4*>(dst + ch) = make_uint4(pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7]));
     };
     if (p.parts == 1) {
         if (softmax && all_fine) {
             const float inv = l_all > 0.0f || l_all != l_all ? 1.0f / l_all : 0.0f;
 #pragma unroll
-            for (int a = 0; a < ND; ++a) {
-                uint32_t ob[32];
-                tmem_ld_32x32(lane_addr + O_COL + (uint32_t)((half * ND + a) * 32), ob);
+            for (int c0 = 0; c0 < HD; c0 += 16) {
+                uint32_t ob[16];
+                tmem_ld_16(lane_addr + O_COL + (uint32_t)(half * HD + c0), ob);
                 if (r < rows) {
 #pragma unroll
-                    for (int c = 0; c < 32; c += 8) {
+                    for (int c = 0; c < 16; c += 8) {
+                        const int ch = half * HD + c0 + c;
                         float x[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(ob[c + i]);
-                        store8((half * ND + a) * 32 + c, x, inv);
+                        store8(ch, x, inv, qpos >= poison[ch >> 5]);
                     }
                 }
             }
@@ -494,11 +550,11 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
         if (softmax) {
             if (n_blocks > 0 && all_fine) {
 #pragma unroll
-                for (int a = 0; a < ND; ++a) {
-                    uint32_t ob[32];
-                    tmem_ld_32x32(lane_addr + O_COL + (uint32_t)((half * ND + a) * 32), ob);
+                for (int c0 = 0; c0 < HD; c0 += 16) {
+                    uint32_t ob[16];
+                    tmem_ld_16(lane_addr + O_COL + (uint32_t)(half * HD + c0), ob);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) state[((half * ND + a) * 32 + i) * QT + r] = __uint_as_float(ob[i]);
+                    for (int i = 0; i < 16; ++i) state[(half * HD + c0 + i) * QT + r] = __uint_as_float(ob[i]);
                 }
             }
             if (half == 0) {
@@ -538,13 +594,7 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
                     asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(key) : "r"(cluster_addr(smem_u32(poison + (ch >> 5)), z)) : "memory");
                     bad = bad || qpos >= key;
                 }
-                if (r < rows && all_fine) {
-                    float y[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) y[i] = bad ? __int_as_float(0x7fc00000) : x[i] * inv;
-                    *reinterpret_cast<uint4*>(dst + ch) =
-                        make_uint4(pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7]));
-                }
+                if (r < rows && all_fine) store8(ch, x, inv, bad);
             }
         }
         cluster_sync_all();                                        // nobody leaves while its results may be read
@@ -595,9 +645,13 @@ int prb_attention_4bit_tile(void* out, long out_stride, const void* q, long q_st
     if (units > 0x7fffffffL / MAX_PARTS) return PRB_E_SIZE;
     Params p{(__nv_bfloat16*)out, out_stride, (const __nv_bfloat16*)q, q_stride, k_tiles, v_tiles, block_table, positions,
              tile_req, tile_row0, tile_rows, tile_count, n_tokens, n_requests, n_tiles, (int)subs, 1, kv_heads, hpg, page_size,
-             max_pages, num_pages, cache4::tile_bytes(head_dim, page_size), scale, status};
+             max_pages, num_pages, cache4::tile_bytes(head_dim, page_size), scale, 0x43004300u, status};
     const int blocks = (max_context + KB - 1) / KB;
-    while (p.parts < MAX_PARTS && units * p.parts < 4L * prb_sm_count() && blocks >= p.parts * 8) p.parts *= 2;
+    // Parts of a tile's keys while all CTAs still run side by side (two an SM at head size 64, one at 128), each of at least
+    // eight blocks: 128 tokens at 1,000 of 12 heads (12 units) 27.7 us in one part, 20.1 in two, 15.7 in four; 2 x 1,024
+    // tokens of 12 heads (192 units) 36.5, 37.5 and 48.1; 512 tokens at 8,000 of 8 x 128 (128 units) 185, 200 and 225.
+    const long slots = (head_dim == 64 ? 2L : 1L) * prb_sm_count();
+    while (p.parts < MAX_PARTS && units * p.parts * 2 <= slots && blocks >= p.parts * 8) p.parts *= 2;
     if (parts > 0) p.parts = parts >= 4 ? 4 : parts >= 2 ? 2 : 1;
     return head_dim == 64 ? launch_tile<1>(p, stream) : launch_tile<2>(p, stream);
 }
