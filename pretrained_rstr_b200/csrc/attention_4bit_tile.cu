@@ -1,5 +1,5 @@
 // Causal attention of prompt portions over a cache held in 4 bits (cache4.cuh) on the 5th-generation tensor cores.
-// bfloat16, head sizes 64 and 128, pages of a multiple of 64 positions, no window.
+// bfloat16, no window; operands are 64 or 128 channels wide, what a head size leaves of them is zero.
 //
 // One CTA takes up to 128 rows (tokens times the query heads of one key/value head) of a tile and walks the keys in
 // blocks of 64, or one of the parts of them (parts are a cluster and meet through distributed shared memory).  Warps:
@@ -33,10 +33,10 @@ constexpr int RAW_STAGES = 3, STAGES = 2, MAX_PARTS = 4;
 constexpr int P_BYTES = QT * KB * 2;
 constexpr float RESCALE_STEP = 8.0f;         // a row's reference maximum moves only by more than this (log2 units)
 
-// ND: head size / 64.
+// ND: operands' width / 64.
 template <int ND> struct Sizes {
     static constexpr int D = 64 * ND, NG = 2 * ND;
-    static constexpr int RAW = KB * (D / 2 + 4 * NG);           // bytes of a block's keys (and of its values)
+    static constexpr int RAW = KB * (D / 2 + 4 * NG);           // most bytes of a block's keys (and of its values)
     static constexpr int TILE = KB * 128;                       // 64 keys x 64 channels of bfloat16
     static constexpr int STAGE = 3 * ND * TILE;                 // keys, what their rounding left, values
     static constexpr int Q_BYTES = QT * D * 2;
@@ -59,7 +59,8 @@ struct Params {
     const int* tile_rows;
     const int* tile_count;
     int n_tokens, n_requests, n_tiles, subs, parts;
-    int kv_heads, hpg, page_size, max_pages, num_pages, tile_bytes;
+    int kv_heads, hpg, head_dim, page_size, max_pages, num_pages, tile_bytes;
+    int piece;                              // keys that lie together in a page and in a block: 64, 32 or 16
     float scale;
     uint32_t magic;                         // 0x43004300: a constant that the compiler keeps in a register
     int* status;
@@ -112,7 +113,8 @@ __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
-template <int ND>
+// FULL: the head size is 64 ND and a block lies in one page, so that the layouts are known here (a tenth of the time).
+template <int ND, bool FULL>
 __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_kernel(const Params p) {
     using Z = Sizes<ND>;
     constexpr int D = Z::D, NG = Z::NG, RAW = Z::RAW, TILE = Z::TILE, STAGE = Z::STAGE;
@@ -167,6 +169,8 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
     const int blk_lo = (int)((long)all_blocks * rank / p.parts);
     const int n_blocks = (int)((long)all_blocks * (rank + 1) / p.parts) - blk_lo;
     const int* table = p.block_table + (size_t)req * p.max_pages;
+    const int head_dim = FULL ? D : p.head_dim, ng = FULL ? NG : cache4::groups_of(head_dim);
+    const int piece = FULL ? KB : p.piece;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < RAW_STAGES; ++s) {
@@ -208,8 +212,16 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
 
     if (warp == 0) {
         // ------------------------------------------------------------------ producer
+        // A block's bytes go where one page of 64 would have them, whatever pages they come from: lane i looks after the page
+        // of piece i, copies (a group's codes, or the pairs, of keys or values of a piece) go around the lanes.
+        const int pieces = KB / piece, row_bytes = head_dim / 2 + 4 * ng, codes_of_page = p.page_size * (head_dim / 2);
+        const int copies = pieces * (ng + 1) * 2;
+        auto page_of = [&](int blk) -> int {
+            const int key = blk * KB + lane * piece;
+            return lane < pieces && key <= pos_hi ? table[key / p.page_size] : -2;       // -2: nothing to fetch
+        };
         int j = 0;
-        int page = n_blocks > 0 ? table[blk_lo * KB / p.page_size] : 0;
+        int page = page_of(blk_lo);
         for (; j < n_blocks; ++j) {
             const int st = j % RAW_STAGES, key0 = (blk_lo + j) * KB;
             ok = mbar_wait_warp(smem_u32(&raw_empty[st]), ((j / RAW_STAGES) & 1) ^ 1, failed);
@@ -219,29 +231,34 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
             }
             const uint32_t fb = smem_u32(&raw_full[st]);
             const bool fine = page >= 0 && page < p.num_pages;
-            const int at = key0 % p.page_size;
-            if (lane == 0) {
-                // (a page that is none: recorded, the stage keeps what it held, and the tile's result is not to be used)
-                if (!fine) prb_set_status(p.status, PRB_S_PAGE_RANGE, row0, key0, page);
-                mbar_expect_tx(fb, fine ? 2 * RAW : 0);
-            }
+            // (a page that is none: recorded, the stage keeps what it held, and the tile's result is not to be used)
+            if (!fine && page != -2) prb_set_status(p.status, PRB_S_PAGE_RANGE, row0, key0 + lane * piece, page);
+            const unsigned who = __ballot_sync(0xffffffffu, fine);
+            if (lane == 0) mbar_expect_tx(fb, (uint32_t)(__popc(who) * 2 * piece * row_bytes));
             __syncwarp();
-            const size_t from = fine ? ((size_t)page * p.kv_heads + hk) * (size_t)p.tile_bytes : 0;
             const uint32_t dst = smem_u32(raw) + st * 2 * RAW;
-            if (fine && p.page_size == KB) {
-                if (lane < 2) bulk_load(dst + lane * RAW, (lane ? p.v_tiles : p.k_tiles) + from, RAW, fb);
-            } else if (fine && lane < 2 * (NG + 1)) {
-                // lane i: copy i / 2 (a group's codes, or the pairs) of keys or values
-                const int c = lane >> 1;
-                const uint8_t* src = (lane & 1 ? p.v_tiles : p.k_tiles) + from;
-                const uint32_t to = dst + (lane & 1) * RAW + c * KB * 16;
-                if (c < NG)
-                    bulk_load(to, src + c * p.page_size * 16 + at * 16, KB * 16, fb);
-                else
-                    bulk_load(to, src + p.page_size * (D / 2) + at * NG * 4, KB * NG * 4, fb);
+            if (p.page_size == KB) {
+                const int pg = __shfl_sync(0xffffffffu, page, 0);
+                if (lane < 2 && (who & 1))
+                    bulk_load(dst + lane * RAW,
+                              (lane ? p.v_tiles : p.k_tiles) + ((size_t)pg * p.kv_heads + hk) * (size_t)p.tile_bytes,
+                              KB * row_bytes, fb);
+            } else {
+                for (int i0 = 0; i0 < copies; i0 += 32) {
+                    const int i = i0 + lane, kind = i & 1, c = (i >> 1) % (ng + 1), pc = min((i >> 1) / (ng + 1), pieces - 1);
+                    const int pg = __shfl_sync(0xffffffffu, page, pc);
+                    if (i < copies && ((who >> pc) & 1)) {
+                        const int in = pc * piece, at = (key0 + in) % p.page_size;
+                        const int row = c == ng ? 4 * ng : min(16, (head_dim - c * 32) / 2);
+                        const uint8_t* src = (kind ? p.v_tiles : p.k_tiles) + ((size_t)pg * p.kv_heads + hk) * (size_t)p.tile_bytes +
+                                             (c == ng ? codes_of_page : c * p.page_size * 16) + at * row;
+                        bulk_load(dst + kind * RAW + (c == ng ? KB * (head_dim / 2) : c * KB * 16) + in * row, src,
+                                  piece * row, fb);
+                    }
+                }
             }
             __syncwarp();
-            if (j + 1 < n_blocks) page = table[(key0 + KB) / p.page_size];
+            if (j + 1 < n_blocks) page = page_of(blk_lo + j + 1);
         }
         if (!ok) {
             for (int jj = j > RAW_STAGES ? j - RAW_STAGES : 0; jj < j; ++jj)      // copies still on their way
@@ -317,12 +334,12 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
         constexpr int HC = KB / 2;
         {
             // the queries, in the layout that a tile copy with the 128-byte swizzle would have made
-            const __nv_bfloat16* src = p.q + (long)(row0 + tk) * p.q_stride + (long)(hk * p.hpg + row - tk * p.hpg) * D;
+            const __nv_bfloat16* src = p.q + (long)(row0 + tk) * p.q_stride + (long)(hk * p.hpg + row - tk * p.hpg) * head_dim;
 #pragma unroll
             for (int c = 0; c < 4 * ND; ++c) {
                 const int ci = half * 4 * ND + c;
                 uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if (row_ok) w = *reinterpret_cast<const uint4*>(src + ci * 8);
+                if (row_ok && ci * 8 < head_dim) w = *reinterpret_cast<const uint4*>(src + ci * 8);
                 st_shared_v4(smem_u32(q_s) + (ci >> 3) * QT * 128 + r * 128 + (((ci & 7) ^ (r & 7)) << 4),
                              __byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632),
                              __byte_perm(w.y, w.w, 0x5410), __byte_perm(w.y, w.w, 0x7632));
@@ -442,8 +459,11 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
 #pragma unroll
             for (int i = 0; i < TASKS; ++i) {
                 const int task = (t >> 5) + i * DEQUANT, g = task >> 3, key = (task & 7) * 8 + key8;
-                word[i] = *reinterpret_cast<const uint32_t*>(src + g * KB * 16 + key * 16 + w * 4);
-                pair[i] = *reinterpret_cast<const uint32_t*>(src + KB * (D / 2) + (key * NG + g) * 4);
+                word[i] = pair[i] = 0u;                                   // (channels beyond the head's are zero)
+                if (g * 32 + w * 8 < head_dim) {
+                    word[i] = *reinterpret_cast<const uint32_t*>(src + g * KB * 16 + key * (head_dim - g * 32 >= 32 ? 16 : 8) + w * 4);
+                    pair[i] = *reinterpret_cast<const uint32_t*>(src + KB * (head_dim / 2) + (key * ng + g) * 4);
+                }
             }
             // (channels i and i + 4 of a word's 8 lie together, as one shift and one mask take them from it: the queries are
             // laid out alike, and the results' channels are put right when they are stored)
@@ -512,7 +532,7 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
     constexpr int HD = D / 2;
     const int row = first + min(r, rows - 1), tk = row / p.hpg, qpos = pos0 + tk;
-    __nv_bfloat16* dst = p.out + (long)(row0 + tk) * p.out_stride + (long)(hk * p.hpg + row - tk * p.hpg) * D;
+    __nv_bfloat16* dst = p.out + (long)(row0 + tk) * p.out_stride + (long)(hk * p.hpg + row - tk * p.hpg) * head_dim;
     // 8 channels from ch on, x in the operands' order (0, 4, 1, 5, 2, 6, 3, 7)
     auto store8 = [&](int ch, const float (&x)[8], float inv, bool bad) {
         const float nan = __int_as_float(0x7fc00000);
@@ -538,7 +558,7 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
                         float x[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(ob[c + i]);
-                        store8(ch, x, inv, qpos >= poison[ch >> 5]);
+                        if (ch < head_dim) store8(ch, x, inv, qpos >= poison[ch >> 5]);
                     }
                 }
             }
@@ -594,7 +614,7 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
                     asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(key) : "r"(cluster_addr(smem_u32(poison + (ch >> 5)), z)) : "memory");
                     bad = bad || qpos >= key;
                 }
-                if (r < rows && all_fine) store8(ch, x, inv, bad);
+                if (r < rows && all_fine && ch < head_dim) store8(ch, x, inv, bad);
             }
         }
         cluster_sync_all();                                        // nobody leaves while its results may be read
@@ -607,8 +627,8 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
     }
 }
 
-template <int ND> int launch_tile(const Params& p, cudaStream_t stream) {
-    cudaError_t e = prb_allow_shared<attention_4bit_tile_kernel<ND>>((int)Sizes<ND>::SMEM);
+template <int ND, bool FULL> int launch_tile(const Params& p, cudaStream_t stream) {
+    cudaError_t e = prb_allow_shared<attention_4bit_tile_kernel<ND, FULL>>((int)Sizes<ND>::SMEM);
     if (e != cudaSuccess) return (int)e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((long)p.n_tiles * p.kv_heads * p.subs * p.parts));
@@ -624,7 +644,7 @@ template <int ND> int launch_tile(const Params& p, cudaStream_t stream) {
     attr[1].val.programmaticStreamSerializationAllowed = prb_small_ctas_early() && prb_pdl_enabled() ? 1 : 0;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, attention_4bit_tile_kernel<ND>, p);
+    e = cudaLaunchKernelEx(&cfg, attention_4bit_tile_kernel<ND, FULL>, p);
     return e == cudaSuccess ? 0 : (int)e;
 }
 }  // namespace
@@ -632,8 +652,8 @@ template <int ND> int launch_tile(const Params& p, cudaStream_t stream) {
 // Whether the tensor-memory kernel takes a call (see prb_attention_4bit).
 bool prb_attention_4bit_tile_takes(int head_dim, int page_size, int window, const void* q, long q_stride, const void* out,
                                    long out_stride) {
-    return (head_dim == 64 || head_dim == 128) && page_size % KB == 0 && window == 0 && (uintptr_t)q % 16 == 0 &&
-           (uintptr_t)out % 16 == 0 && q_stride % 8 == 0 && out_stride % 8 == 0;
+    return cache4::takes(head_dim, page_size) && window == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 &&
+           q_stride % 8 == 0 && out_stride % 8 == 0;
 }
 
 int prb_attention_4bit_tile(void* out, long out_stride, const void* q, long q_stride, const uint8_t* k_tiles,
@@ -644,14 +664,17 @@ int prb_attention_4bit_tile(void* out, long out_stride, const void* q, long q_st
     const long subs = (rows + QT - 1) / QT, units = (long)n_tiles * kv_heads * subs;
     if (units > 0x7fffffffL / MAX_PARTS) return PRB_E_SIZE;
     Params p{(__nv_bfloat16*)out, out_stride, (const __nv_bfloat16*)q, q_stride, k_tiles, v_tiles, block_table, positions,
-             tile_req, tile_row0, tile_rows, tile_count, n_tokens, n_requests, n_tiles, (int)subs, 1, kv_heads, hpg, page_size,
-             max_pages, num_pages, cache4::tile_bytes(head_dim, page_size), scale, 0x43004300u, status};
+             tile_req, tile_row0, tile_rows, tile_count, n_tokens, n_requests, n_tiles, (int)subs, 1, kv_heads, hpg, head_dim,
+             page_size, max_pages, num_pages, cache4::tile_bytes(head_dim, page_size),
+             page_size % 64 == 0 ? 64 : page_size % 32 == 0 ? 32 : 16, scale, 0x43004300u, status};
     const int blocks = (max_context + KB - 1) / KB;
     // Parts of a tile's keys while all CTAs still run side by side (two an SM at head size 64, one at 128), each of at least
     // eight blocks: 128 tokens at 1,000 of 12 heads (12 units) 27.7 us in one part, 20.1 in two, 15.7 in four; 2 x 1,024
     // tokens of 12 heads (192 units) 36.5, 37.5 and 48.1; 512 tokens at 8,000 of 8 x 128 (128 units) 185, 200 and 225.
-    const long slots = (head_dim == 64 ? 2L : 1L) * prb_sm_count();
+    const long slots = (head_dim <= 64 ? 2L : 1L) * prb_sm_count();
     while (p.parts < MAX_PARTS && units * p.parts * 2 <= slots && blocks >= p.parts * 8) p.parts *= 2;
     if (parts > 0) p.parts = parts >= 4 ? 4 : parts >= 2 ? 2 : 1;
-    return head_dim == 64 ? launch_tile<1>(p, stream) : launch_tile<2>(p, stream);
+    if (p.piece == KB && head_dim == 64) return launch_tile<1, true>(p, stream);
+    if (p.piece == KB && head_dim == 128) return launch_tile<2, true>(p, stream);
+    return head_dim <= 64 ? launch_tile<1, false>(p, stream) : launch_tile<2, false>(p, stream);
 }

@@ -177,6 +177,12 @@ CASES = [
     ([1000], [128], 1, 1, 64, 128, None),
     ([700, 63], [65, 129], 2, 1, 128, 192, None),
     ([0], [50], 40, 1, 64, 64, None),
+    ([11, 200], [40, 70], 4, 4, 16, 16, None),
+    ([100], [60], 3, 3, 32, 48, None),
+    ([33, 5], [50, 34], 2, 1, 48, 32, None),
+    ([90], [64], 3, 3, 80, 16, None),
+    ([150], [40], 4, 2, 96, 96, None),
+    ([20], [129], 2, 2, 112, 48, None),
 ]
 
 
@@ -186,7 +192,7 @@ CASES = [
 def test_attention_against_64_bits(case, parts, dtype):
     ops = _ops()
     held, new, heads, kv, d, page, window = CASES[case]
-    if parts in (1, 3) and case not in (1, 3, 5, 13, 17, 19):
+    if parts in (1, 3) and case not in (1, 3, 5, 13, 17, 19, 24, 27):
         pytest.skip("one or two long cases are enough for a forced number of parts")
     g = torch.Generator().manual_seed(case)
     total = [a + n for a, n in zip(held, new)]
@@ -226,7 +232,8 @@ def test_attention_against_64_bits(case, parts, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("heads,kv,d,page,new", [(2, 2, 64, 64, 80), (4, 1, 128, 64, 30), (2, 1, 96, 32, 40), (1, 1, 64, 64, 3)])
+@pytest.mark.parametrize("heads,kv,d,page,new", [(2, 2, 64, 64, 80), (4, 1, 128, 64, 30), (2, 1, 96, 32, 40), (1, 1, 64, 64, 3),
+                                                  (2, 2, 80, 16, 40)])
 @pytest.mark.parametrize("parts", [0, 1, 4])
 def test_a_token_that_is_no_number_reaches_those_that_see_it(heads, kv, d, page, new, dtype, parts):
     """A NaN among a token's keys makes that token's and all later results NaN in the heads that share it; one among its
