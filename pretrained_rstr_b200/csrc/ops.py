@@ -2722,13 +2722,13 @@ def _ints(what: str, name: str, t, n: int) -> int:
     return t.data_ptr()
 
 
-def _matrix4(what: str, name: str, t, rows: int, width: int) -> int:
-    """The row stride of [>= rows, width] with neighbouring columns."""
+def _matrix4(what: str, name: str, t, rows: int, width: int, written: bool = False) -> int:
+    """The row stride of [>= rows, width] with neighbouring columns; rows that are written do not overlap."""
     if t.dim() != 2:
         raise KernelArgumentError(f"{what}: {name} must be [tokens, {width}], is {list(t.shape)}")
     n, w = t.shape
     stride, step = t.stride()
-    if w != width or n < rows or (step != 1 and width > 1) or stride < 0:
+    if w != width or n < rows or (step != 1 and width > 1) or stride < 0 or (written and n > 1 and stride < width):
         raise KernelArgumentError(f"{what}: {name} must be [tokens, {width}] with neighbouring columns and at least "
                                   f"{rows} rows, is {list(t.shape)}")
     return stride
@@ -2810,8 +2810,8 @@ def kv_read_4bit(k_out, v_out, k_tiles, v_tiles, slots, n_tokens: int, head_dim:
     if n_tokens < 0:
         raise KernelArgumentError(f"{what}: n_tokens is below zero")
     width = heads * head_dim
-    k_stride = _matrix4(what, "k_out", k_out, n_tokens, width)
-    v_stride = _matrix4(what, "v_out", v_out, n_tokens, width)
+    k_stride = _matrix4(what, "k_out", k_out, n_tokens, width, True)
+    v_stride = _matrix4(what, "v_out", v_out, n_tokens, width, True)
     _launch_on(device, what, "prb_kv_read_4bit", k_out.data_ptr(), k_stride, v_out.data_ptr(), v_stride,
                k_tiles.data_ptr(), v_tiles.data_ptr(), _ints(what, "slots", slots, n_tokens), n_tokens, heads, head_dim,
                page_size, pages, _code4(what, "k_out", "v_out", k_out, v_out),
@@ -2824,7 +2824,8 @@ def attention_4bit(out, q, k_tiles, v_tiles, block_table, positions, tile_req, t
     """Causal attention of tiles of tokens over their requests' pages of a cache held in 4 bits
     (:func:`kv_append_4bit`), the tokens' own keys and values included.
 
-    ``q``, ``out``: [T, n_heads * head_dim], both bfloat16 or both float32 (may be column slices); ``block_table``
+    ``q``, ``out``: [T, n_heads * head_dim], both bfloat16 or both float32, of memory of their own (may be column
+    slices of one tensor); ``block_table``
     int32 [requests, pages a request]; ``positions`` int32 [T].  Tile i: tokens ``tile_row0[i]`` to ``tile_row0[i] +
     tile_rows[i] - 1``, neighbours of request ``tile_req[i]`` (a row of the block table) at neighbouring positions;
     no tile has more than ``tile_most`` of them, and 128 rows (tokens times the heads that share a key/value head) a
@@ -2855,7 +2856,7 @@ def attention_4bit(out, q, k_tiles, v_tiles, block_table, positions, tile_req, t
     width = n_heads * head_dim
     q_stride = _matrix4(what, "q", q, 0, width)
     tokens = q.shape[0]
-    out_stride = _matrix4(what, "out", out, tokens, width)
+    out_stride = _matrix4(what, "out", out, tokens, width, True)
     code = _code4(what, "q", "out", q, out)
     q_at, out_at = q.data_ptr(), out.data_ptr()
     if q_at == out_at and tokens > 0:
@@ -2915,7 +2916,7 @@ def step_tables(rows, held, brought, tables, page_size: int, q_start, kv_len, po
     t_at, b_at = _ints(what, "tables", tables, 0), _ints(what, "block_table", block_table, 0)
     if t_at < b_at + 4 * n * wide and b_at < t_at + 4 * lanes * wide:
         raise KernelArgumentError(f"{what}: block_table and tables are two tensors")
-    free_at, start_at, next_at, n_free = None, None, None, 0
+    free_at, start_at, next_at, n_free = None, None, None, -1
     if free_pages is not None:
         if free_start is None or free_next is None:
             raise KernelArgumentError(f"{what}: free_pages come with free_start and free_next")

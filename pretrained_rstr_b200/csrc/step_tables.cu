@@ -35,7 +35,8 @@ struct TableArgs {
     int* seq_of_token;
     int* slots;
     int* block_table;
-    int n_requests, n_rows, t_cap, max_pages, page_size, n_free;
+    int n_requests, n_rows, t_cap, max_pages, page_size;
+    int n_free;                              // below zero: no list, the rows hold their pages already
     int* status;
 };
 
@@ -65,7 +66,7 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const TableArgs p)
             else prb_set_status(p.status, PRB_S_POSITION_RANGE, b, held, brought);
         }
         const int w = fine ? (int)(((long)held + brought + p.page_size - 1) / p.page_size) : -1;
-        const int h = !fine ? -1 : p.free_pages != nullptr ? (int)(((long)held + p.page_size - 1) / p.page_size) : w;
+        const int h = !fine ? -1 : p.n_free >= 0 ? (int)(((long)held + p.page_size - 1) / p.page_size) : w;
         have[b] = h;
         tok[b] = t_sum;                      // (within the thread's run, for now)
         fresh[b] = f_sum;
@@ -111,7 +112,7 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const TableArgs p)
         fresh[p.n_requests] = f_total;
     }
     __syncthreads();
-    const int start = p.free_start != nullptr ? *p.free_start : 0;
+    const int start = p.n_free >= 0 ? *p.free_start : 0;
     auto free_page = [&](int b, int i) -> int {              // the i-th page that b takes
         const long at = (long)start + fresh[b] + i;
         return at >= 0 && at < p.n_free ? p.free_pages[at] : -1;
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const TableArgs p)
         if (threadIdx.x == 0) {
             p.q_start[p.n_requests] = min(t_total, p.t_cap);
             if (t_total > p.t_cap) prb_set_status(p.status, PRB_S_ROW_RANGE, -1, t_total, p.t_cap);
-            if (p.free_next != nullptr) *p.free_next = start + f_total;
+            if (p.n_free >= 0) *p.free_next = add(max(start, 0), f_total);
             if (f_total > 0 && (start < 0 || (long)start + f_total > p.n_free))
                 prb_set_status(p.status, PRB_S_PAGE_RANGE, -1, start + f_total, p.n_free);
         }
@@ -177,9 +178,10 @@ PRB_API int prb_step_tables(const int* rows, const int* held, const int* brought
                             int* seq_of_token, int* slots, int* block_table, int n_requests, int n_rows, int t_cap,
                             int max_pages, int page_size, int n_free, int* status, cudaStream_t stream) {
     if (n_requests <= 0 || n_requests > MAX_REQUESTS || n_rows <= 0 || t_cap < 0 || t_cap > MOST || max_pages <= 0 ||
-        page_size <= 0 || n_free < 0 || (long)max_pages * page_size > 0x7fffffffL)
+        page_size <= 0 || (long)max_pages * page_size > 0x7fffffffL)
         return PRB_E_SIZE;
-    if (n_free > 0 && (free_pages == nullptr || free_start == nullptr)) return PRB_E_ARG;
+    if (n_free >= 0 && (free_start == nullptr || free_next == nullptr || (n_free > 0 && free_pages == nullptr)))
+        return PRB_E_ARG;
     const TableArgs a{rows, held, brought, tables, free_pages, free_start, free_next, q_start, kv_len, positions,
                       seq_of_token, slots, block_table, n_requests, n_rows, t_cap, max_pages, page_size, n_free, status};
     const int shared = (3 * n_requests + 2) * (int)sizeof(int);

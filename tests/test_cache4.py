@@ -60,6 +60,28 @@ def test_the_plain_verification_follows_the_rule():
     assert plain.verify(logits, [0, 2], [0, 0], [[0.5, 0.8], [0.0, 0.0]], [0.0]) == ([0, 2], [1])
 
 
+@pytest.mark.parametrize("group", [1, 2, 4, 8, 40])
+def test_tiles_of_a_step(group):
+    """Every token of a step lies in one tile of its request, in order; short ones in the list of few rows."""
+    import numpy as np
+    from pretrained_rstr_b200.parts.attention import Attention4Work
+    work = Attention4Work(group)
+    lengths = [1, 130, 8, 9, 1, 300, 2, 128]
+    room = {n: np.full(words, fill, np.int32) for n, (words, fill) in work.arrays(sum(lengths), len(lengths)).items()}
+    counts = work.fill(room, lengths)
+    seen = []
+    for name, counter, most in (("few", "few", work.few_most), ("tile", "tiles", work.tile_most)):
+        for i in range(counts[counter]):
+            req, row, n = (int(room[f"{name}_{part}"][i]) for part in ("req", "row0", "rows"))
+            assert 1 <= n <= most and n * group <= (max(8, group) if name == "few" else max(128, group))
+            seen += [(t, req) for t in range(row, row + n)]
+        assert set(room[f"{name}_req"][counts[counter]:]) <= {-1}
+    assert sorted(seen) == list(enumerate(b for b, n in enumerate(lengths) for _ in range(n)))
+    assert counts["few"] == sum(1 for n in lengths if n <= work.few_most)
+    one = work.fill({n: np.full(words, fill, np.int32) for n, (words, fill) in work.arrays(8, 8).items()}, [1] * 8)
+    assert one["tiles"] == 0 and one["few"] == 8 and one["_used"] == ["few_req", "few_row0", "few_rows"]
+
+
 # ------------------------------------------------------------------------------------ refusals
 # (shapes and types are looked at before the library is asked for anything: no device is needed to be refused)
 class _FakeCuda(torch.Tensor):
@@ -99,7 +121,7 @@ def _append_args(**kw):
     (dict(k_tiles=fake(4, 2, 100, dtype=torch.uint8)), "k_tiles"), (dict(status=fake(2)), "status"),
     (dict(v_tiles=fake(3, 2, plain.tile_bytes(16, 32), dtype=torch.uint8)), "differ in shape"),
     (dict(k=torch.zeros(5, 64, dtype=torch.bfloat16)), "not on a CUDA device"),
-    (dict(n_tokens=-1), "n_tokens")])
+    (dict(n_tokens=-1), "n_tokens"), (dict(k=fake(1, 64, dtype=torch.bfloat16).expand(5, 64), n_tokens=6), "k must be")])
 def test_rows_refused(ops, change, word):
     with pytest.raises(ops.KernelArgumentError, match=word):
         ops.kv_append_4bit(**_append_args(**change))
@@ -129,7 +151,7 @@ _Q = fake(6, 128, dtype=torch.bfloat16)
     (dict(window=-3), "window"), (dict(tile_count=fake(0)), "tile_count"), (dict(block_table=fake(7)), "block_table"),
     (dict(block_table=fake(3, 7, dtype=torch.int64)), "block_table"), (dict(q=_Q, out=_Q), "out must not be q"),
     (dict(tile_most=0), "tile_most"), (dict(max_context=0), "max_context"), (dict(parts=9), "parts"),
-    (dict(scale=math.nan), "scale"), (dict(head_dim=40), "multiples of 16")])
+    (dict(out=fake(1, 128, dtype=torch.bfloat16).expand(6, 128)), "out must be"), (dict(scale=math.nan), "scale"), (dict(head_dim=40), "multiples of 16")])
 def test_attention_refused(ops, change, word):
     with pytest.raises(ops.KernelArgumentError, match=word):
         ops.attention_4bit(**_attention_args(**change))

@@ -265,6 +265,58 @@ def test_a_token_that_is_no_number_reaches_those_that_see_it(heads, kv, d, page,
     assert torch.equal(out[0][~nan], out[1][~nan])
 
 
+def _call(seed, page_offset=0, pool=None, dtype=torch.bfloat16, new=1):
+    """Append, read back, attend for two requests; all inputs from ``seed``.  Pages ``page_offset`` ... of ``pool``."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(seed)
+    kv, d, page, total = 8, 128, 64, [130, 70]
+    pages = [[page_offset + 3, page_offset, page_offset + 4], [page_offset + 1, page_offset + 2, -1]]
+    tile = plain.tile_bytes(page, d)
+    kt, vt = pool or [torch.zeros(6, kv, tile, dtype=torch.uint8, device=CUDA) for _ in range(2)]
+    n = sum(total)
+    x = torch.randn(n, 3 * kv * d, generator=g).to(dtype).to(CUDA)
+    q, k, v = x[:, :kv * d], x[:, kv * d:2 * kv * d], x[:, 2 * kv * d:]
+    slots = _ints([pages[b][i // page] * page + i % page for b, t in enumerate(total) for i in range(t)])
+    status = _status()
+    ops.kv_append_4bit(kt, vt, k, v, slots, n, d, page, status)
+    back = [torch.zeros(n, kv * d, device=CUDA) for _ in range(2)]
+    ops.kv_read_4bit(*back, kt, vt, slots, n, d, page, status)
+    positions = _ints([i for t in total for i in range(t)])
+    at = [129, 199] if new == 1 else [130 - new, 200 - new]
+    out = torch.zeros(n, kv * d, dtype=dtype, device=CUDA)
+    ops.attention_4bit(out, q, kt, vt, _ints(pages), positions, _ints([0, 1]), _ints(at), _ints([new, new]), new, kv, d, page,
+                       0.1, None, 130, status)
+    return back + [out, status]
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_pages_beyond_four_gigabytes(new):
+    """The last pages of a pool of 4.7 GB of keys (and of values) give the bits that the first ones of a small pool give."""
+    tile, last = plain.tile_bytes(64, 128), 115000
+    pool = [torch.empty(last + 6, 8, tile, dtype=torch.uint8, device=CUDA) for _ in range(2)]
+    for a, b in zip(_call(1, new=new), _call(1, last, pool, new=new)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new", [1, 40])
+def test_calls_on_two_streams_at_once(dtype, new):
+    """No call shares memory with another: two streams' calls give what they give alone."""
+    alone = [_call(seed, dtype=dtype, new=new) for seed in (1, 2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(_call(i + 1, dtype=dtype, new=new))
+    torch.cuda.synchronize()
+    for want, runs in zip(alone, got):
+        for run in runs:
+            for a, b in zip(want, run):
+                assert torch.equal(a, b)
+
+
 # --------------------------------------------------------------------------------------- tables
 def _run_tables(rows, held, brought, table, page, cap, free=None, start=0):
     ops = _ops()
@@ -319,6 +371,9 @@ def test_step_tables_report_what_does_not_fit():
     assert status[0] in (2, 4)
     got, status = _run_tables([0], [15], [3], table, 16, 30, free=[9], start=1)
     assert status[0] == 4 and got[4][:3] == [4 * 16 + 15, -1, -1] and got[5] == [[4, -1]]
+    # an empty list is a list: what a request grows into is missing
+    got, status = _run_tables([0], [15], [3], [[4, 9], [6, 7]], 16, 30, free=[], start=0)
+    assert status[0] == 4 and got[4][:3] == [4 * 16 + 15, -1, -1] and got[7] == 1
     # more tokens than rows: those behind are left out
     got, status = _run_tables([1, 0], [0, 0], [20, 3], table, 16, 21)
     assert status[0] == 6 and got[0] == [0, 20, 21] and got[4][20] == 64
@@ -328,7 +383,7 @@ def test_step_tables_report_what_does_not_fit():
 @pytest.mark.parametrize("draft", ["probabilities", "tokens"])
 @pytest.mark.parametrize("requests,drafts,vocab,temperature", [
     (1, 0, 7, 1.0), (1, 3, 1, 0.7), (3, 4, 50257, 0.8), (5, 2, 501, 1.3), (2, 31, 999, 1.0), (9, 3, 50257, 0.0),
-    (40, 5, 130, 0.5)])
+    (40, 5, 130, 0.5), (2, 2, 70001, 1.0), (3, 1, 131072, 0.9)])
 def test_verify_drafts(requests, drafts, vocab, temperature, draft):
     ops = _ops()
     g = torch.Generator().manual_seed(requests * 100 + drafts)
