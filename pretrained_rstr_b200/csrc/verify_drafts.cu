@@ -281,45 +281,70 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, 4) veri
             return all;
         };
         const bool keep = each <= KEPT;
+        if (q != nullptr)                                                 // (wanted once the sum below is known)
+            for (int i = lo + 32 * threadIdx.x; i < hi; i += 32 * THREADS)
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i));
         auto raw = [&](int i) -> double { return exp64(((double)x[i] - (double)top) * inverse); };
-        double z = 0.0;
-        for (int i0 = w0 + lane; i0 < w1; i0 += 32 * AHEAD) {
-            float v[AHEAD];
+        double v = 0.0;
+        float ahead[AHEAD];
 #pragma unroll
-            for (int k = 0; k < AHEAD; ++k) v[k] = i0 + 32 * k < w1 ? x[i0 + 32 * k] : -INFINITY;
+        for (int k = 0; k < AHEAD; ++k) ahead[k] = w0 + lane + 32 * k < w1 ? x[w0 + lane + 32 * k] : -INFINITY;
+        for (int i0 = w0 + lane; i0 < w1; i0 += 32 * AHEAD) {
+            float l[AHEAD];
 #pragma unroll
             for (int k = 0; k < AHEAD; ++k) {
-                const double e = exp64(((double)v[k] - (double)top) * inverse);
+                l[k] = ahead[k];
+                ahead[k] = i0 + 32 * (k + AHEAD) < w1 ? x[i0 + 32 * (k + AHEAD)] : -INFINITY;
+            }
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const double e = exp64(((double)l[k] - (double)top) * inverse);
                 if (keep && i0 + 32 * k < w1) kept_e[i0 + 32 * k - lo] = e;
-                z += e;
+                v += e;
             }
         }
-        z = 1.0 / meet(z);
-        auto weight = [&](int i, bool less) -> double {
-            const double w = (keep ? kept_e[i - lo] : raw(i)) * z;
-            if (!less) return w;
-            if (q != nullptr) return fmax(w - (double)q[i], 0.0);
-            return i == gone ? 0.0 : w;
-        };
+        double whole = meet(v);
+        // Behind a refused token: what the target's probability leaves over the draft's, in the kept ones' place.  Without one
+        // the exponentials are the weights as they are.
+        const double z = 1.0 / whole;
         bool less = refused;
-        double whole = 0.0;
-        for (int go = 0; go < 2; ++go) {
-            double v = 0.0;
-            if (less && q != nullptr && keep) {
-                for (int i0 = w0 + lane; i0 < w1; i0 += 32 * AHEAD) {
-                    float said[AHEAD];
+        auto weight = [&](int i) -> double {
+            if (keep) return kept_e[i - lo];
+            const double e = raw(i);
+            if (!less) return e;
+            if (q != nullptr) return fmax(e * z - (double)q[i], 0.0);
+            return i == gone ? 0.0 : e;
+        };
+        if (less) {
+            v = 0.0;
+            for (int i0 = w0 + lane; i0 < w1; i0 += 32 * AHEAD) {
+                float said[AHEAD];
 #pragma unroll
-                    for (int k = 0; k < AHEAD; ++k) said[k] = i0 + 32 * k < w1 ? q[i0 + 32 * k] : 0.0f;
+                for (int k = 0; k < AHEAD; ++k) said[k] = q != nullptr && keep && i0 + 32 * k < w1 ? q[i0 + 32 * k] : 0.0f;
 #pragma unroll
-                    for (int k = 0; k < AHEAD; ++k)
-                        if (i0 + 32 * k < w1) v += fmax(kept_e[i0 + 32 * k - lo] * z - (double)said[k], 0.0);
+                for (int k = 0; k < AHEAD; ++k) {
+                    const int i = i0 + 32 * k;
+                    if (i >= w1) break;
+                    if (keep) {
+                        const double e = kept_e[i - lo], w = q != nullptr ? fmax(e * z - (double)said[k], 0.0) : i == gone ? 0.0 : e;
+                        kept_e[i - lo] = w;
+                        v += w;
+                    } else {
+                        v += weight(i);
+                    }
                 }
-            } else {
-                for (int i = w0 + lane; i < w1; i += 32) v += weight(i, less);
             }
             whole = meet(v);
-            if (whole > 0.0 || !less) break;
-            less = false;                                                 // nothing left: the target's own
+            if (!(whole > 0.0)) {                                         // nothing left: the target's own
+                less = false;
+                v = 0.0;
+                for (int i = w0 + lane; i < w1; i += 32) {
+                    const double e = raw(i);
+                    if (keep) kept_e[i - lo] = e;
+                    v += e;
+                }
+                whole = meet(v);
+            }
         }
         const double want = (double)p.uniforms[2 * row + 1] * whole;
         // the CTA whose sums pass it, else the last that has any weight
@@ -353,24 +378,40 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, 4) veri
             const bool inside = mine >= 0;
             if (!inside) mine = final_mine;
             if (mine == warp) {
-                double sum = mine_before;
-                int found = -1, final_token = w0;
-                for (int i0 = w0; i0 < w1 && found < 0; i0 += 32) {
-                    const int i = i0 + lane;
-                    const double w = i < w1 ? weight(i, less) : 0.0;
-                    double up = w;
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const double v = __shfl_up_sync(0xffffffffu, up, o);
-                        if (lane >= o) up += v;
-                    }
-                    const unsigned over = __ballot_sync(0xffffffffu, inside && w > 0.0 && sum + up > want);
-                    const unsigned any = __ballot_sync(0xffffffffu, w > 0.0);
-                    if (any) final_token = i0 + 31 - __clz(any);
-                    if (over) found = i0 + __ffs(over) - 1;
-                    sum += __shfl_sync(0xffffffffu, up, 31);
+                // each lane a run of neighbours (of an odd length: no bank of shared memory twice at a time), then the lane
+                // whose sums pass it goes through its own
+                const int each_lane = ((w1 - w0 + 31) / 32) | 1;
+                const int a = min(w0 + lane * each_lane, w1), b1 = min(a + each_lane, w1);
+                double own = 0.0;
+                int final_token = -1;
+                for (int i = a; i < b1; ++i) {
+                    const double w = weight(i);
+                    own += w;
+                    if (w > 0.0) final_token = i;
                 }
-                if (lane == 0) p.tokens[row] = found >= 0 ? found : final_token;
+                double up = own;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double below = __shfl_up_sync(0xffffffffu, up, o);
+                    if (lane >= o) up += below;
+                }
+                const unsigned over = __ballot_sync(0xffffffffu, inside && final_token >= 0 && mine_before + up > want);
+                const unsigned any = __ballot_sync(0xffffffffu, final_token >= 0);
+                // (rounding may leave nobody that passes it: then the last token with any weight)
+                const int chosen_lane = over ? __ffs(over) - 1 : any ? 31 - __clz(any) : 0;
+                if (lane == chosen_lane) {
+                    int found = final_token < 0 ? 0 : final_token;
+                    double sum = mine_before + (up - own);
+                    for (int i = a; over && i < b1; ++i) {
+                        const double w = weight(i);
+                        sum += w;
+                        if (w > 0.0 && sum > want) {
+                            found = i;
+                            break;
+                        }
+                    }
+                    p.tokens[row] = found;
+                }
             }
         }
     } else if (rank == 0 && threadIdx.x == 0) {
