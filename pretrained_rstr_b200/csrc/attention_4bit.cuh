@@ -39,8 +39,15 @@ constexpr int MAX_WARPS = 4;
 constexpr int STAGES = 2;                  // ring buffers of a warp
 constexpr int MAX_PARTS = 8;               // CTAs of a cluster (portable)
 
-// keys of a stage: 64, or 32 where a warp's buffers or its scores would grow too large
-__host__ __device__ constexpr int stage_keys(int ng, int qn) { return ng <= 2 && qn <= 2 ? 64 : 32; }
+// Keys of a stage: 64, or 32 where a thread's scores and results would not fit the registers.  Longer stages and more
+// registers measured better than more warps: 8 x 32,749 positions of 8 x 128 87.5 us with stages of 32 keys and four CTAs an
+// SM, 78.6 with 64 and two; 64 tokens at 1,000 of 25 heads of 64 42 with 64, 51 with 32.
+__host__ __device__ constexpr int stage_keys(int ng, int qn, bool wide) {
+    return (ng <= 2 && qn <= 2) || (qn == 1 && !wide) ? 64 : 32;
+}
+
+// CTAs of four warps that an SM takes (by their registers).
+__host__ __device__ constexpr int ctas_of(int ng, int qn, bool wide) { return qn > 1 ? 2 : ng > 2 ? (wide ? 3 : 2) : 4; }
 
 struct Args {
     void* out;
@@ -181,8 +188,8 @@ template <int NG> __device__ __forceinline__ void load_params(const uint8_t* p, 
         for (int g = 0; g < NG; ++g) out[g] = reinterpret_cast<const uint32_t*>(p)[g];
     }
 }
-template <int NG, int QN, int EN> struct Layout {
-    static constexpr int SK = stage_keys(NG, QN), ROWS = EN == 1 ? 4 : 8 * QN;
+template <int NG, int QN, int EN, typename T> struct Layout {
+    static constexpr int SK = stage_keys(NG, QN, sizeof(T) == 4), ROWS = EN == 1 ? 4 : 8 * QN;
     static constexpr int DP = NG * 32, PART = DP + 2;         // floats a row of a partial state: values, maximum, sum
     static constexpr int KIND = SK * (16 * NG + 4 * NG);      // most bytes of a stage's keys (and of its values)
     static constexpr int STAGE = 2 * KIND;
@@ -196,9 +203,9 @@ template <int NG, int QN, int EN> struct Layout {
 // row's scores rather than two.  FAST: the head size is 32 NG and a stage lies in one page, so that every offset is known
 // here.
 template <int NG, int QN, int EN, typename T, bool FAST>
-__global__ void __launch_bounds__(MAX_WARPS * 32, QN > 1 ? 2 : NG > 2 && sizeof(T) == 4 ? 3 : 4)
+__global__ void __launch_bounds__(MAX_WARPS * 32, ctas_of(NG, QN, sizeof(T) == 4))
 attention_4bit_kernel(const Args p) {
-    using L = Layout<NG, QN, EN>;
+    using L = Layout<NG, QN, EN, T>;
     constexpr int SK = L::SK, ROWS = L::ROWS, NC = SK / 16, DP = L::DP, PART = L::PART;
     constexpr int PIECES = sizeof(T) == 4 ? 3 : 1;
     constexpr bool EXACT = PIECES == 3;                       // codes less 8 in the keys' products too
@@ -748,7 +755,7 @@ attention_4bit_kernel(const Args p) {
 }
 
 template <int NG, int QN, int EN, typename T, bool FAST> int launch_one(const Args& p, cudaStream_t stream) {
-    using L = Layout<NG, QN, EN>;
+    using L = Layout<NG, QN, EN, T>;
     cudaError_t e = prb_allow_shared<attention_4bit_kernel<NG, QN, EN, T, FAST>>(L::bytes(MAX_WARPS));
     if (e != cudaSuccess) return (int)e;
     cudaLaunchConfig_t cfg = {};
@@ -771,24 +778,25 @@ template <int NG, int QN, int EN, typename T, bool FAST> int launch_one(const Ar
 
 // `p` but for subs, parts, warps and piece is set; rows: the most rows of a tile.
 template <int NG, int QN, int EN, typename T> int launch_by(Args p, long rows, int max_context, int parts, cudaStream_t stream) {
-    constexpr int sk = stage_keys(NG, QN);
+    constexpr int sk = stage_keys(NG, QN, sizeof(T) == 4);
     p.piece = p.page_size % sk == 0 ? sk : p.page_size % 32 == 0 ? 32 : 16;
     if (sk % p.page_size == 0) p.piece = p.page_size;
-    constexpr int most = Layout<NG, QN, EN>::ROWS;
+    constexpr int most = Layout<NG, QN, EN, T>::ROWS;
     const long subs = (rows + most - 1) / most, units = (long)p.n_tiles * p.kv_heads * subs;
     if (units > 0x7fffffffL / MAX_PARTS) return PRB_E_SIZE;
     p.subs = (int)subs;
-    // Four warps a CTA; two once the units alone fill the SMs with four such CTAs each: a warp then has twice the stages to
+    // Four warps a CTA; two once the units alone fill the SMs with such CTAs: a warp then has twice the stages to
     // one set-up and half as many states to merge.  64 tokens at 1,000 of 12 heads (768 units) 27.9 us with four, 23.3 with
     // two; at 300 of 16 heads (1,024) 15.6 and 13.6; 24 x 5 tokens of 16 heads (384) 14.4 and 19.7; float32 texts (more
     // instructions a stage) 30.9 and 39.8.
-    p.warps = QN == 1 && sizeof(T) == 2 && units > 4L * prb_sm_count() ? 2 : MAX_WARPS;
-    // Parts of a unit's keys: as many as give every SM about four CTAs, each with a stage a warp at least.  (The longest
+    const long slots = (long)ctas_of(NG, QN, sizeof(T) == 4) * prb_sm_count();
+    p.warps = QN == 1 && sizeof(T) == 2 && units > slots ? 2 : MAX_WARPS;
+    // Parts of a unit's keys while all CTAs still run side by side, each with a stage a warp at least.  (The longest
     // request's: max_context, or what a window and the tile's own tokens span.)
     const int reach = p.window > 0 ? min((long)max_context, (long)p.window + p.tile_most + sk) : max_context;
     const int stages = (reach + sk - 1) / sk + (p.window > 0 ? 1 : 0);   // (a window need not begin with a stage)
     p.parts = 1;
-    while (p.parts < MAX_PARTS && units * p.parts * 2 <= 4L * prb_sm_count() && stages >= p.parts * 2 * p.warps) p.parts *= 2;
+    while (p.parts < MAX_PARTS && units * p.parts * 2 <= slots && stages >= p.parts * 2 * p.warps) p.parts *= 2;
     if (parts > 0) p.parts = parts;
     if (p.piece == sk && p.head_dim == 32 * NG) return launch_one<NG, QN, EN, T, true>(p, stream);
     return launch_one<NG, QN, EN, T, false>(p, stream);
