@@ -13,6 +13,12 @@
 // query's and the key's lengths times it, which at ordinary scores is several times what P's rounding costs, and the tensor
 // cores wait for the softmax anyway.
 //
+// Measured: portions of 4 x 512 tokens at contexts of 4,000, 16 heads of 64 (16.5 GFLOP) 102 us, where tiles of 32 rows on
+// mma.sync take 207; 512 tokens at 8,000 of 32 heads over 8 x 128 (65 GFLOP) 190 us, 340 TFLOP/s.  What bounds it: the
+// instructions of softmax and conversion (6,500 a block of 64 keys, a third of them the conversion, in 70 % of the issue
+// slots while a CTA pair runs), and the SMs that one tile less leaves with one CTA where others have two.  Eight warps
+// convert: with four the blocks waited for them (512 tokens at 8,000: 302 us).
+//
 // What lies behind the tile's last position (stale pages, NaN) becomes zeros.  A key that the tile's later tokens see and
 // its earlier ones do not may read back as NaN: it becomes zeros too, and the rows that see it are made NaN in the channels
 // of its group at the end, since a product would spread it over all rows.
@@ -260,12 +266,11 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
             __syncwarp();
             if (j + 1 < n_blocks) page = page_of(blk_lo + j + 1);
         }
-        if (!ok) {
-            for (int jj = j > RAW_STAGES ? j - RAW_STAGES : 0; jj < j; ++jj)      // copies still on their way
-                for (uint32_t i = 0; i < WAIT_LIMIT; ++i)
-                    if (mbar_try_wait(smem_u32(&raw_full[jj % RAW_STAGES]), (jj / RAW_STAGES) & 1)) break;
-            __syncwarp();
-        }
+        // copies still on their way, whoever has given up: nobody leaves before they have landed
+        for (int jj = j > RAW_STAGES ? j - RAW_STAGES : 0; jj < j; ++jj)
+            for (uint32_t i = 0; i < WAIT_LIMIT; ++i)
+                if (mbar_try_wait(smem_u32(&raw_full[jj % RAW_STAGES]), (jj / RAW_STAGES) & 1)) break;
+        __syncwarp();
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer
         constexpr uint32_t idesc_s = make_idesc(QT, KB);          // queries, keys: both K-major

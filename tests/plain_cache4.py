@@ -169,10 +169,11 @@ def tiles_of(lengths: Sequence[int], most: int):
 
 def attention_bound(ref, terms, keys: int, dtype) -> torch.Tensor:
     """How far a result may be from the 64-bit one.  bfloat16: half a step of the result (2^-8), of every probability
-    times its step (2^-8 of A) and of every probability that goes with a middle (2^-8 of B - A), so 2^-8 of B.  Both types: a score that 32-bit sums moved by E moves a probability by up
-    to 2 E of itself (once by itself, once by the sum of all; e^x - 1 <= 1.01 x here), the exponential is good for
-    2^-21 with its argument's rounding (2^-24 of up to 64 log2 units), and sums over the keys one after the other lose up
-    to 2^-23 a key."""
+    times its step (2^-8 of A) and of every probability that goes with a middle (2^-8 of B - A), so 2^-8 of B.  Both
+    types: a score that 32-bit sums moved by E moves a probability by up to 2 E of itself (once by itself, once by the sum
+    of all; e^x - 1 <= 1.01 x here), the exponential is good for 2^-21 with its argument's rounding (2^-24 of up to 64 log2
+    units), and sums over the keys one after the other lose up to 2^-23 a key.  (Portions of prompts round values too,
+    another 2^-8 of p |value|: they are held to the same bound, which the roundings' signs leave room for.)"""
     _a, b, e = terms
     assert float(e.max()) < 0.01
     wide = 2 * (1.01 * e + 2.0 ** -21 + 2.0 ** -17) + (keys + 16) * 2.0 ** -23
