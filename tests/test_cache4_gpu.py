@@ -183,6 +183,8 @@ CASES = [
     ([90], [64], 3, 3, 80, 16, None),
     ([150], [40], 4, 2, 96, 96, None),
     ([20], [129], 2, 2, 112, 48, None),
+    # more heads to a key/value head than a tile has rows
+    ([20], [2], 130, 1, 16, 16, None),
 ]
 
 
@@ -263,6 +265,39 @@ def test_a_token_that_is_no_number_reaches_those_that_see_it(heads, kv, d, page,
     nan[bad_v - held:, heads - group:, (d - 1) // 32 * 32:] = True
     assert torch.equal(torch.isnan(out[1]), nan)
     assert torch.equal(out[0][~nan], out[1][~nan])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new", [1, 40])
+def test_what_a_tile_may_not_name_is_reported(new, dtype):
+    """A page that is none, a request, a row, a position or a tile that does not fit: recorded, and the other request's
+    results are what they are without it.  ``tile_count`` leaves the tiles behind it alone."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(new)
+    kt, vt = (plain.pack(*plain.quantize(torch.randn(6, 2, 64, 64, generator=g))).to(CUDA) for _ in range(2))
+    q = torch.randn(2 * new, 128, generator=g).to(dtype).to(CUDA)
+
+    def go(table=((0, 1, -1), (2, 3, -1)), positions=None, req=(0, 1), row0=(0, new), n=(new, new), most=new, count=None):
+        out, status = torch.zeros(2 * new, 128, dtype=dtype, device=CUDA), _status()
+        at = list(range(85, 85 + new)) + list(range(80, 80 + new)) if positions is None else positions
+        ops.attention_4bit(out, q, kt, vt, _ints([list(r) for r in table]), _ints(at), _ints(list(req)), _ints(list(row0)),
+                           _ints(list(n)), most, 2, 64, 64, 0.1, None, 192, status,
+                           tile_count=None if count is None else _ints([count]))
+        return out, status.tolist()
+    want, status = go()
+    assert status == [0] * 4
+    for kw, code in ((dict(table=((0, -1, -1), (2, 3, -1))), 4), (dict(table=((0, 6, -1), (2, 3, -1))), 4),
+                     (dict(req=(2, 1)), 2), (dict(req=(-1, 1)), 2), (dict(row0=(-1, new)), 2), (dict(row0=(new + 1, new)), 2),
+                     (dict(positions=[200] * new + list(range(80, 80 + new))), 2)):
+        out, status = go(**kw)
+        assert status[0] == code, (kw, status)
+        assert torch.equal(out[new:], want[new:]), kw
+    out, status = go(count=1)
+    assert status == [0] * 4 and torch.equal(out[:new], want[:new]) and not out[new:].any()
+    out, status = go(count=0)
+    assert status == [0] * 4 and not out.any()
+    out, status = go(n=(0, new))
+    assert status == [0] * 4 and not out[:new].any() and torch.equal(out[new:], want[new:])
 
 
 def _call(seed, page_offset=0, pool=None, dtype=torch.bfloat16, new=1):
