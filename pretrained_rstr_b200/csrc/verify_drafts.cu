@@ -19,8 +19,8 @@
 // 256 threads, so that four CTAs fit an SM and the clusters of 64 requests run side by side.
 //
 // 64 requests of 5 rows of 50,257: 42 us, of which a CTA spends 13 to 17 on the rows (64 MB are 10 us' worth), 5 on who stays
-// and 15 on the drawn row, where it waits for the others three times; without a draw (temperature 0) 23 us.  One request
-// of 5 rows 19.5 us, of which 10 on the drawn row.
+// and 15 on the drawn row, where it waits for the others three times; without a draw (temperature 0) 22 us.  One request
+// of 5 rows 19 us, of which 10 on the drawn row.
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -115,7 +115,9 @@ __device__ __forceinline__ double exp64(double x) {
     return y * __hiloint2double((1023 + (int)k) << 20, 0);
 }
 
-__global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, 4) verify_kernel(const VerifyArgs p) {
+// AHEAD_ROWS: the next row's logits are asked for before a row is worked on, for launches that leave the registers for it.
+template <bool AHEAD_ROWS>
+__global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, AHEAD_ROWS ? 2 : 4) verify_kernel(const VerifyArgs p) {
     __shared__ Shared s;
     extern __shared__ double kept_e[];       // [each] exponentials of the row that is drawn from
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -138,8 +140,36 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, 4) veri
     const int lo = min(rank * each, p.vocab), hi = min(lo + each, p.vocab);
 
     // ---------------------------------------------------------- every row: maximum, sum
+    // 16 bytes at a time from the first such border on; up to three logits before it and behind the last one alone
+    auto head_of = [&](int r) -> int {
+        const float* x = p.logits + (long)(r0 + r) * p.logits_stride + lo;
+        return min((int)((16 - ((uintptr_t)x & 15)) & 15) / 4, hi - lo);
+    };
+    // a thread's part of a row, all asked for before the first is used; -inf weighs nothing
+    auto batch = [&](int r, int i, float (&v)[4 * BATCH]) {
+        const int head = head_of(r), vecs = (hi - lo - head) / 4;
+        const float4* body = reinterpret_cast<const float4*>(p.logits + (long)(r0 + r) * p.logits_stride + lo + head);
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            float4 w = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (i + k * THREADS < vecs) w = body[i + k * THREADS];
+            v[4 * k] = w.x; v[4 * k + 1] = w.y; v[4 * k + 2] = w.z; v[4 * k + 3] = w.w;
+        }
+    };
+    auto edge = [&](int r, float& v) -> int {
+        const int head = head_of(r), tail = lo + head + (hi - lo - head) / 4 * 4;
+        const int at = threadIdx.x < 4 ? (threadIdx.x < head ? lo + threadIdx.x : hi)
+                                       : threadIdx.x < 8 ? min(tail + (int)threadIdx.x - 4, hi) : hi;
+        v = at < hi ? p.logits[(long)(r0 + r) * p.logits_stride + at] : -INFINITY;
+        return at;
+    };
+    float v[4 * BATCH], lone;
+    int lone_at = 0;
+    if (AHEAD_ROWS) {
+        batch(0, threadIdx.x, v);
+        lone_at = edge(0, lone);
+    }
     for (int r = 0; r < rows; ++r) {
-        const float* x = p.logits + (long)(r0 + r) * p.logits_stride;
         float top = -INFINITY, sum = 0.0f;
         int index = 0x7fffffff;
         auto sums = [&](const auto& v) {
@@ -153,34 +183,43 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, 4) veri
             for (int i = 0; i < n; ++i) sum += exp2_fast((v[i] - ref) * scale);
             top = now;
         };
-        // 16 bytes at a time from the first such border on; up to three logits before it and behind the last one alone
-        const int head = min((int)((16 - ((uintptr_t)(x + lo) & 15)) & 15) / 4, hi - lo);
-        const int vecs = (hi - lo - head) / 4, tail = lo + head + 4 * vecs;
-        const float4* body = reinterpret_cast<const float4*>(x + lo + head);
-        for (int i = threadIdx.x; i < vecs; i += BATCH * THREADS) {
-            float v[4 * BATCH];                              // (all asked for before the first is used; -inf weighs nothing)
-#pragma unroll
-            for (int k = 0; k < BATCH; ++k) {
-                float4 w = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                if (i + k * THREADS < vecs) w = body[i + k * THREADS];
-                v[4 * k] = w.x; v[4 * k + 1] = w.y; v[4 * k + 2] = w.z; v[4 * k + 3] = w.w;
-            }
-            if (greedy) {
-#pragma unroll
-                for (int k = 0; k < BATCH; ++k)
-                    if (i + k * THREADS < vecs) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) better(top, index, v[4 * k + e], lo + head + 4 * (i + k * THREADS) + e);
-                    }
-            } else {
+        const int head = head_of(r), vecs = (hi - lo - head) / 4;
+        auto take = [&](const float (&v)[4 * BATCH], int i) {
+            if (!greedy) {
                 sums(v);
+                return;
             }
+#pragma unroll
+            for (int k = 0; k < BATCH; ++k)
+                if (i + k * THREADS < vecs) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) better(top, index, v[4 * k + e], lo + head + 4 * (i + k * THREADS) + e);
+                }
+        };
+        float next[4 * BATCH], next_lone = -INFINITY;
+        int next_at = hi;
+        if (!AHEAD_ROWS) {
+            batch(r, threadIdx.x, v);
+            lone_at = edge(r, lone);
+        } else if (r + 1 < rows) {
+            batch(r + 1, threadIdx.x, next);
+            next_at = edge(r + 1, next_lone);
         }
-        const int lone = threadIdx.x < 4 ? (threadIdx.x < head ? lo + threadIdx.x : hi) : tail + threadIdx.x - 4;
-        if (threadIdx.x < 8 && lone < hi) {
-            const float v[1] = {x[lone]};
-            if (greedy) better(top, index, v[0], lone);
-            else sums(v);
+        take(v, threadIdx.x);
+        for (int i = threadIdx.x + BATCH * THREADS; i < vecs; i += BATCH * THREADS) {
+            batch(r, i, v);
+            take(v, i);
+        }
+        if (lone_at < hi) {
+            const float one[1] = {lone};
+            if (greedy) better(top, index, lone, lone_at);
+            else sums(one);
+        }
+        if (AHEAD_ROWS) {
+#pragma unroll
+            for (int i = 0; i < 4 * BATCH; ++i) v[i] = next[i];
+            lone = next_lone;
+            lone_at = next_at;
         }
         // the warp's lanes
         const float own = top;
@@ -439,9 +478,16 @@ PRB_API int prb_verify_drafts(int* tokens, int* accepted, const float* logits, l
     const VerifyArgs a{tokens, accepted, logits, logits_stride, row_start, drafted, draft_probs, probs_stride, uniforms,
                        temperature, n_requests, n_rows, vocab, status};
     const int each = (vocab + PARTS - 1) / PARTS;
-    cudaError_t e = prb_allow_shared<verify_kernel>(KEPT * (int)sizeof(double));
+    const size_t shared = each <= KEPT ? each * sizeof(double) : 0;
+    // The next row asked for ahead takes 110 registers instead of 62, so it is for launches of two CTAs an SM at most.  us
+    // without and with it, 50,257 logits a row: 1 request of 4 rows, greedy, 8.9 and 8.0; 32 of them 11.8 and 10.1; 32 of 5
+    // rows at temperature 0.8 32.0 and 26.8; but 64 of those, where four CTAs an SM do more, 41.2 and 51.2.
+    const bool ahead = (long)n_requests * PARTS <= 2L * prb_sm_count();
+    cudaError_t e = ahead ? prb_allow_shared<verify_kernel<true>>(KEPT * (int)sizeof(double))
+                          : prb_allow_shared<verify_kernel<false>>(KEPT * (int)sizeof(double));
     if (e != cudaSuccess) return (int)e;
-    e = prb_launch_dependent(verify_kernel, dim3((unsigned)n_requests * PARTS), dim3(THREADS),
-                             each <= KEPT ? each * sizeof(double) : 0, stream, a);
+    const dim3 grid((unsigned)n_requests * PARTS);
+    e = ahead ? prb_launch_dependent(verify_kernel<true>, grid, dim3(THREADS), shared, stream, a)
+              : prb_launch_dependent(verify_kernel<false>, grid, dim3(THREADS), shared, stream, a);
     return e == cudaSuccess ? 0 : (int)e;
 }
