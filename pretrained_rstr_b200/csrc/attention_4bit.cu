@@ -1,5 +1,6 @@
 // Causal attention over a cache held in 4 bits: the launch, and the bfloat16 form of the kernel in attention_4bit.cuh.
 #include "attention_4bit.cuh"
+#include "ranges.cuh"
 
 // (attention_4bit_tile.cu, attention_4bit_f32.cu, attention_4bit_rows.cu)
 bool prb_attention_4bit_tile_takes(int head_dim, int page_size, int window, const void* q, long q_stride, const void* out,
@@ -48,6 +49,8 @@ PRB_API int prb_attention_4bit(void* out, long out_stride, const void* q, long q
     if ((uintptr_t)k_tiles % 16 != 0 || (uintptr_t)v_tiles % 16 != 0) return PRB_E_ALIGN;
     if (dtype != PRB_F32 && dtype != PRB_BF16) return PRB_E_DTYPE;
     const int size = dtype == PRB_F32 ? 4 : 2, hpg = heads / kv_heads;
+    if (!prb_rows_apart(out, out_stride * size, q, q_stride * size, n_tokens, (long)heads * head_dim * size))
+        return PRB_E_OVERLAP;
     attn4::Args p{};
     p.out = out; p.out_stride = out_stride; p.q = q; p.q_stride = q_stride;
     p.k_tiles = (const uint8_t*)k_tiles; p.v_tiles = (const uint8_t*)v_tiles;

@@ -12,6 +12,7 @@
 // difference's own rounding left out behind it.  Step and middle are taken in 64 bits, two operations a group.
 // A group that holds an infinity or a NaN reads back as NaN.
 #include "cache4.cuh"
+#include "ranges.cuh"
 
 namespace {
 using cache4::GROUP;
@@ -181,6 +182,11 @@ int launch_rows(bool append, RowArgs a, int dtype, cudaStream_t stream) {
         if ((uintptr_t)a.tiles[i] % 16 != 0) return PRB_E_ALIGN;
         wide = wide && (uintptr_t)a.rows[i] % 16 == 0 && (a.stride[i] * size) % 16 == 0;
     }
+    const long pool = a.num_pages * (long)a.heads * cache4::tile_bytes(a.head_dim, a.page_size);
+    if (append ? prb_overlap({a.tiles[0], pool}, {a.tiles[1], pool})
+               : !prb_rows_apart(a.rows[0], a.stride[0] * size, a.rows[1], a.stride[1] * size, a.n_tokens,
+                                 (long)a.heads * a.head_dim * size))
+        return PRB_E_OVERLAP;
     a.groups = cache4::groups_of(a.head_dim);
     const int threads_of_token = append ? 2 * a.heads * a.groups * 4 : 2 * a.heads * (a.head_dim / 8);
     // (as few CTAs a token as its threads need, of equal size)

@@ -19,6 +19,7 @@
 #define PRB_E_SIZE (-3)      // a size the kernel does not take
 #define PRB_E_ALIGN (-4)     // a pointer or stride that is not aligned as required
 #define PRB_E_ARG (-5)       // any other bad argument
+#define PRB_E_OVERLAP (-7)   // memory that is written lies over other memory of the call
 
 // element type codes shared with Python
 #define PRB_F32 0

@@ -26,6 +26,7 @@ _ERRORS = {
     -4: "a pointer or stride that is not aligned as the kernel requires",
     -5: "bad argument",
     -6: "the device or driver lacks a feature the kernel needs",
+    -7: "memory that is written overlaps another tensor of the call",
 }
 STATUS_TEXT = {
     1: "token id outside the vocabulary (token index, id, vocabulary size)",
@@ -2776,7 +2777,7 @@ def kv_append_4bit(k_tiles, v_tiles, k, v, slots, n_tokens: int, head_dim: int, 
     """Round the step's keys and values to 4 bits at their cache slots.  ``k_tiles`` / ``v_tiles``: uint8 [pages,
     kv_heads, ``cache4_tile_bytes(head_dim, page_size)``]; ``k`` / ``v``: [T, kv_heads * head_dim] bfloat16 or float32,
     may be column slices of a wider tensor; ``slots`` int32: page * page_size + place of each token, below zero = none.
-    No two tokens have one slot.
+    No two tokens have one slot, and the two tensors of tiles are two.
 
     Of every 32 channels (the last group may be shorter) the cache keeps step = (largest - smallest) / 15 and middle =
     smallest + 8 step in bfloat16 and per channel the nearest of 16 codes; code c reads back as middle + step * (c - 8).
@@ -2887,7 +2888,8 @@ def step_tables(rows, held, brought, tables, page_size: int, q_start, kv_len, po
     ``tables`` too; ``free_next[0]`` becomes the place behind the last one taken (not ``free_start`` itself: the caller
     has the two take turns).  What a row holds behind its request's ``held`` tokens is overwritten, not used: where
     requests give tokens back (refused drafts), their pages are better reserved beforehand.  Without ``free_pages`` the
-    rows of ``tables`` hold the pages already (the cache manager reserves them on the host).
+    rows of ``tables`` hold the pages already (the cache manager reserves them on the host).  No tensor that is written
+    shares memory with another one (the new lengths cannot take the place of ``held``).
 
     In the status word: a request whose row or lengths do not fit (it brings nothing, its block table row stays
     empty), a page that is missing (the slot is -1), more tokens than token rows (those behind are left out)."""
@@ -2946,7 +2948,7 @@ def verify_drafts(tokens, accepted, logits, row_start, drafted, uniforms, temper
     drafted token, the lowest index at which the running sum passes the number's share of the whole.
 
     Written: ``accepted[b]``: drafted tokens that stay; ``tokens`` int32 [rows]: they and the token behind them, -1 in
-    the request's rows beyond."""
+    the request's rows beyond.  Neither shares memory with another tensor of the call."""
     what = "verify_drafts"
     device = logits.get_device()
     if device < 0 or tokens.get_device() != device or accepted.get_device() != device or \

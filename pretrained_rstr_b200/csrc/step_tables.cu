@@ -15,6 +15,7 @@
 // by whoever needs it rather than read back from the table.  Rows of `tables` beyond what a request held are written
 // by one CTA each and read by none.
 #include "common.cuh"
+#include "ranges.cuh"
 
 namespace {
 constexpr int THREADS = 256;
@@ -182,6 +183,14 @@ PRB_API int prb_step_tables(const int* rows, const int* held, const int* brought
         return PRB_E_SIZE;
     if (n_free >= 0 && (free_start == nullptr || free_next == nullptr || (n_free > 0 && free_pages == nullptr)))
         return PRB_E_ARG;
+    // (a CTA may still read what another writes: the new lengths, for one, must not take the place of those held)
+    const long word = sizeof(int), n = n_requests, table = n_rows * (long)max_pages;
+    if (!prb_apart({{q_start, (n + 1) * word}, {kv_len, n * word}, {positions, t_cap * word}, {seq_of_token, t_cap * word},
+                    {slots, t_cap * word}, {block_table, n * max_pages * word}, {tables, table * word},
+                    {n_free >= 0 ? free_next : nullptr, word}},
+                   {{rows, n * word}, {held, n * word}, {brought, n * word}, {free_pages, n_free * word},
+                    {n_free >= 0 ? free_start : nullptr, word}}))
+        return PRB_E_OVERLAP;
     const TableArgs a{rows, held, brought, tables, free_pages, free_start, free_next, q_start, kv_len, positions,
                       seq_of_token, slots, block_table, n_requests, n_rows, t_cap, max_pages, page_size, n_free, status};
     const int shared = (3 * n_requests + 2) * (int)sizeof(int);

@@ -22,6 +22,7 @@
 // and 15 on the drawn row, where it waits for the others three times; without a draw (temperature 0) 22 us.  One request
 // of 5 rows 19 us, of which 10 on the drawn row.
 #include "common.cuh"
+#include "ranges.cuh"
 #include "tcgen05.cuh"
 
 namespace {
@@ -475,6 +476,12 @@ PRB_API int prb_verify_drafts(int* tokens, int* accepted, const float* logits, l
                               cudaStream_t stream) {
     if (n_requests <= 0 || n_rows <= 0) return 0;
     if (vocab <= 0 || n_requests > 0x7fffffff / PARTS) return PRB_E_SIZE;
+    const long word = 4, width = vocab * word;
+    if (!prb_apart({{tokens, n_rows * word}, {accepted, n_requests * word}},
+                   {{row_start, (n_requests + 1) * word}, {drafted, n_rows * word}, {uniforms, 2 * n_rows * word},
+                    {temperature, n_requests * word}, {logits, prb_span(n_rows, logits_stride * word, width)},
+                    {draft_probs, prb_span(n_rows, probs_stride * word, width)}}))
+        return PRB_E_OVERLAP;
     const VerifyArgs a{tokens, accepted, logits, logits_stride, row_start, drafted, draft_probs, probs_stride, uniforms,
                        temperature, n_requests, n_rows, vocab, status};
     const int each = (vocab + PARTS - 1) / PARTS;

@@ -201,3 +201,61 @@ _W = fake(6)
 def test_verification_refused(ops, change, word):
     with pytest.raises(ops.KernelArgumentError, match=word):
         ops.verify_drafts(**_verify_args(**change))
+
+
+# Tensors that share memory: the library itself refuses them, before it asks for a device.
+@pytest.fixture
+def real_ops(monkeypatch):
+    from pretrained_rstr_b200.csrc import ops as module
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda _d: 0, raising=False)
+    return module
+
+
+@pytest.mark.parametrize("ours,theirs", [
+    ("kv_len", "held"), ("kv_len", "brought"), ("kv_len", "rows"), ("q_start", "held"), ("slots", "positions"),
+    ("positions", "seq_of_token"), ("free_next", "held"), ("block_table", "free_pages"), ("kv_len", "q_start")])
+@pytest.mark.parametrize("behind", [0, 2])
+def test_tables_that_share_memory_are_refused(real_ops, ours, theirs, behind):
+    a = _table_args()
+    pool = fake(64)
+    if behind and a[theirs].numel() <= behind:
+        behind = 0
+    for name, at in ((theirs, 8), (ours, 8 + behind)):
+        a[name] = pool[at:at + a[name].numel()].view(a[name].shape)
+    with pytest.raises(real_ops.KernelArgumentError, match="overlaps"):
+        real_ops.step_tables(**a)
+
+
+@pytest.mark.parametrize("ours,theirs", [("accepted", "row_start"), ("accepted", "drafted"), ("tokens", "row_start"),
+                                         ("tokens", "accepted"), ("tokens", "uniforms"), ("accepted", "temperature"),
+                                         ("tokens", "logits"), ("accepted", "draft_probs")])
+def test_verification_of_shared_memory_is_refused(real_ops, ours, theirs):
+    a = _verify_args()
+    a[ours] = a[theirs].view(torch.int32).flatten()[-a[ours].numel():] if a[theirs].numel() >= a[ours].numel() else a[ours]
+    if a[theirs].numel() < a[ours].numel():
+        a[theirs] = a[ours][:a[theirs].numel()].view(a[theirs].dtype)
+    with pytest.raises(real_ops.KernelArgumentError, match="overlaps"):
+        real_ops.verify_drafts(**a)
+
+
+@pytest.mark.parametrize("q_at,out_at,stride", [(0, 256, 256), (256, 0, 256), (0, 64, 256), (64, 0, 256), (0, 192, 256),
+                                                (0, 512 + 100, 256)])
+def test_attention_rows_that_share_memory_are_refused(real_ops, q_at, out_at, stride):
+    pool = fake(4096, dtype=torch.bfloat16)
+
+    def rows(at):
+        return pool.as_strided((6, 128), (stride, 1), at)
+    with pytest.raises(real_ops.KernelArgumentError, match="overlaps"):
+        real_ops.attention_4bit(**_attention_args(q=rows(q_at), out=rows(out_at)))
+
+
+def test_cache_rows_that_share_memory_are_refused(real_ops):
+    a = _append_args()
+    with pytest.raises(real_ops.KernelArgumentError, match="overlaps"):
+        real_ops.kv_append_4bit(**dict(a, v_tiles=a["k_tiles"]))
+    rows = fake(5, 100, dtype=torch.bfloat16)
+    back = {k: v for k, v in a.items() if k not in "kv"}
+    for v_out in (rows[:, :64], rows[:, 36:]):
+        with pytest.raises(real_ops.KernelArgumentError, match="overlaps"):
+            real_ops.kv_read_4bit(k_out=rows[:, :64], v_out=v_out, **back)

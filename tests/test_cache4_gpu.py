@@ -324,6 +324,30 @@ def _call(seed, page_offset=0, pool=None, dtype=torch.bfloat16, new=1):
     return back + [out, status]
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new", [1, 40])
+def test_results_beside_the_queries_in_one_tensor(new, dtype):
+    """q and out as neighbouring columns of one tensor give the bits that tensors of their own give; q stays as it was."""
+    ops = _ops()
+    kv, d, page = 4, 64, 64
+    g = torch.Generator().manual_seed(3)
+    kt, vt = [torch.zeros(2, kv, plain.tile_bytes(page, d), dtype=torch.uint8, device=CUDA) for _ in range(2)]
+    k, v, q = [torch.randn(100, kv * d, generator=g).to(dtype).to(CUDA) for _ in range(3)]
+    status = _status()
+    ops.kv_append_4bit(kt, vt, k, v, _ints(list(range(100))), 100, d, page, status)
+    both = torch.zeros(100, 2 * kv * d, dtype=dtype, device=CUDA)
+    for at in (0, kv * d):
+        other = kv * d - at
+        both[:, at:at + kv * d] = q
+        both[:, other:other + kv * d] = 0
+        alone = torch.zeros(100, kv * d, dtype=dtype, device=CUDA)
+        for q_in, out in ((q, alone), (both[:, at:at + kv * d], both[:, other:other + kv * d])):
+            ops.attention_4bit(out, q_in, kt, vt, _ints([[0, 1]]), _ints(list(range(100))), _ints([0]), _ints([100 - new]),
+                               _ints([new]), new, kv, d, page, 0.125, None, 100, status)
+        assert alone[100 - new:].abs().sum() > 0 and status.tolist() == [0] * 4
+        assert torch.equal(both[:, other:other + kv * d], alone) and torch.equal(both[:, at:at + kv * d], q)
+
+
 @pytest.mark.parametrize("new", [1, 40])
 def test_pages_beyond_four_gigabytes(new):
     """The last pages of a pool of 4.7 GB of keys (and of values) give the bits that the first ones of a small pool give."""
@@ -418,7 +442,8 @@ def test_step_tables_report_what_does_not_fit():
 @pytest.mark.parametrize("draft", ["probabilities", "tokens"])
 @pytest.mark.parametrize("requests,drafts,vocab,temperature", [
     (1, 0, 7, 1.0), (1, 3, 1, 0.7), (3, 4, 50257, 0.8), (5, 2, 501, 1.3), (2, 31, 999, 1.0), (9, 3, 50257, 0.0),
-    (40, 5, 130, 0.5), (2, 2, 70001, 1.0), (3, 1, 131072, 0.9)])
+    (40, 5, 130, 0.5), (2, 2, 70001, 1.0), (3, 1, 131072, 0.9),
+    (38, 2, 60001, 0.9), (75, 4, 5003, 0.0)])
 def test_verify_drafts(requests, drafts, vocab, temperature, draft):
     ops = _ops()
     g = torch.Generator().manual_seed(requests * 100 + drafts)
