@@ -88,11 +88,11 @@ class Model:
                 raise ValueError(f"run order: layer {e.layer} reads the cache of layer "
                                  f"{e.cache_layer}, which no entry writes")
         keyed: Dict[Tuple, List[int]] = {}
+        wanted = getattr(self.runtime, "cache_bits", None)
         for layer in sorted(writers):
             mixer = self.blocks[owner[layer]].mixer
             spec = mixer.kv_spec()
             if spec is not None:
-                wanted = getattr(self.runtime, "cache_bits", None)
                 if spec.bits != wanted:
                     raise ValueError(f"cache_bits={wanted}: layer {layer}'s mixer ({type(mixer).__name__}) keeps its "
                                      f"cache in the runtime's type only")
@@ -100,6 +100,8 @@ class Model:
                                   2 if spec.values else 1, spec.bits), []).append(layer)
             for st in mixer.state_specs():
                 self.state_specs[(layer, st.name)] = st
+        if wanted is not None and not keyed:
+            raise ValueError(f"cache_bits={wanted}: this design caches no keys and values")
         for st in self.embedding.state_specs() if hasattr(self.embedding, "state_specs") else ():
             self.state_specs[(-1, st.name)] = st            # (-1: the embedding's own state)
         for (kv_heads, head_dim, window, pools, bits), layers in sorted(
@@ -114,10 +116,10 @@ class Model:
             reader = self.blocks[e.layer].mixer.kv_spec()
             if reader is not None and e.cache_layer in self.layer_group:
                 g = self.group_specs[self.layer_group[e.cache_layer][0]]
-                if (reader.kv_heads, reader.head_dim, 2 if reader.values else 1) != \
-                        (g.kv_heads, g.head_dim, g.pools_per_layer):
+                if (reader.kv_heads, reader.head_dim, 2 if reader.values else 1, reader.bits) != \
+                        (g.kv_heads, g.head_dim, g.pools_per_layer, g.bits):
                     raise ValueError(f"run order: layer {e.layer} cannot read the cache of layer "
-                                     f"{e.cache_layer}: head counts or sizes differ")
+                                     f"{e.cache_layer}: head counts, sizes or bits differ")
 
     def attach_storage(self, storage) -> None:
         """Bind every run entry to the pages and state tensors of its cache layer."""

@@ -259,3 +259,30 @@ def test_cache_rows_that_share_memory_are_refused(real_ops):
     for v_out in (rows[:, :64], rows[:, 36:]):
         with pytest.raises(real_ops.KernelArgumentError, match="overlaps"):
             real_ops.kv_read_4bit(k_out=rows[:, :64], v_out=v_out, **back)
+
+
+# ------------------------------------------------------------------------------------ layout of a model's caches
+def _layout(bits, specs, readers=()):
+    """A model of one layer a spec, and of layers that read the cache of layer 0: only its layout is derived."""
+    from types import SimpleNamespace as Some
+    from pretrained_rstr_b200.models.assembly import Model
+    blocks = [Some(mixer=Some(kv_spec=lambda s=s: s, state_specs=lambda: ())) for s in (*specs, *readers)]
+    order = [Some(layer=i, cache_layer=i if i < len(specs) else 0, writes_cache=i < len(specs)) for i in range(len(blocks))]
+    m = Some(runtime=Some(cache_bits=bits), order=order, blocks=blocks, embedding=object(), state_specs={}, group_specs=[],
+             layer_group={})
+    Model._derive_cache_layout(m)
+    return m
+
+
+def test_layout_of_caches_in_4_bits():
+    from pretrained_rstr_b200.parts.interfaces import KVSpec
+    four, plain_kv = KVSpec(4, 64, bits=4), KVSpec(4, 64)
+    assert [g.bits for g in _layout(4, [four, four], [four]).group_specs] == [4]
+    assert [g.bits for g in _layout(None, [plain_kv], [plain_kv]).group_specs] == [None]
+    with pytest.raises(ValueError, match="runtime's type only"):
+        _layout(4, [four, plain_kv])
+    with pytest.raises(ValueError, match="bits differ"):
+        _layout(4, [four], [plain_kv])
+    with pytest.raises(ValueError, match="no keys and values"):
+        _layout(4, [None])
+    assert _layout(None, [None]).group_specs == []
