@@ -435,10 +435,11 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(p_full));
         }
-        // the row sum: both halves
-        xmax[half * QT + r] = l_run;
+        // the row sum: both halves, in the words of a block behind the last: the other thread may not have read the last
+        // block's maximum yet
+        xmax[((n_blocks & 1) * 2 + half) * QT + r] = l_run;
         asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");
-        l_all = half == 0 ? l_run + xmax[QT + r] : xmax[r] + l_run;
+        l_all = l_run + xmax[((n_blocks & 1) * 2 + (half ^ 1)) * QT + r];
         if (ok && n_blocks > 0) ok = mbar_wait_warp(smem_u32(o_full), (n_blocks - 1) & 1, failed);
         tcgen05_fence_after();
         if (!ok && lane == 0) prb_set_status(p.status, PRB_S_WAIT_TIMEOUT, 45, blockIdx.x, warp);

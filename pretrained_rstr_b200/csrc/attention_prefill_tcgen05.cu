@@ -499,10 +499,11 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q,
 #ifdef PRB_TRACE
         if (warp == 2 && lane == 0) PF_CTA(3, pf_now());
 #endif
-        // the row sum: both halves (every thread of the pair reaches this barrier)
-        xmax[half * QT + r] = l_run;
+        // the row sum: both halves, in the words of a block behind the last (the other thread may not have read the
+        // last block's maximum yet; every thread of the pair reaches this barrier)
+        xmax[((n_blocks & 1) * 2 + half) * QT + r] = l_run;
         asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");
-        const float l_all = half == 0 ? l_run + xmax[QT + r] : xmax[r] + l_run;
+        const float l_all = l_run + xmax[((n_blocks & 1) * 2 + (half ^ 1)) * QT + r];
         if (ok) {
             ok = mbar_wait(smem_u32(o_full), (n_blocks - 1) & 1, failed);
             ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;

@@ -74,3 +74,27 @@ def test_the_first_kernel_behind_the_page_copies_is_launched_the_plain_way():
     for entry in ("prb_embed(", "prb_copy_pages("):
         body = code.split("PRB_API int " + entry, 1)[1].split("PRB_API", 1)[0]
         assert "<<<" in body and "prb_launch" not in body
+
+
+@pytest.mark.parametrize("name", ["attention_4bit_tile.cu", "attention_prefill_tcgen05.cu"])
+def test_two_threads_of_a_row_overwrite_no_word_that_the_other_may_still_read(name):
+    """Two threads share a row of the prompt kernels: a block's maxima, and the sums in the end, go through words of
+    shared memory with one barrier between the writes and the reads.  So what a thread writes behind a barrier lies
+    apart from what the other reads behind the same one, for every number of blocks."""
+    code = _code(name)
+    writes = re.findall(r"xmax\[([^;]*)\] = ", code)
+    reads = re.findall(r"[^;]*;", code[code.index(writes[0]):])
+    reads = [m for part in reads if "xmax[" in part for m in re.findall(r"xmax\[([^;]*?)\](?! = )(?=[);\s:])", part)]
+    assert len(writes) == 2 and 2 <= len(reads) <= 3
+
+    def words(expressions, half, j, n_blocks):
+        return {eval(e, {"half": half, "j": j, "n_blocks": n_blocks, "QT": 128, "r": 5}) for e in expressions}
+    for n_blocks in range(0, 9):
+        # (what is written before a barrier, what is read behind it) of the two halves, barrier after barrier
+        steps = [[(words(writes[:1], h, j, n_blocks), words(reads[:1], h, j, n_blocks)) for h in (0, 1)] for j in range(n_blocks)]
+        steps.append([(words(writes[1:], h, 0, n_blocks), words(reads[1:], h, 0, n_blocks)) for h in (0, 1)])
+        for now, then in zip(steps, steps[1:]):
+            for h in (0, 1):
+                assert not now[h][1] & then[1 - h][0], (n_blocks, h)
+        for step in steps:
+            assert all(step[h][1] - step[h][0] <= step[1 - h][0] for h in (0, 1))
