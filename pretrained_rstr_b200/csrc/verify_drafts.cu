@@ -8,7 +8,7 @@
 //   refused (from p, should nothing be left), from p behind the last drafted one: the lowest index at which the
 //   running sum passes v times the whole.
 // Without probabilities of the draft q is 1 at the drafted token.  Temperature 0 or less: a token stays while it is the
-// largest logit (the lowest index among equals), and the largest logit follows.
+// largest logit (the lowest index among equals, a NaN before all numbers), and the largest logit follows.
 //
 // One launch; a cluster of eight CTAs takes a request, each an eighth of the vocabulary, and they meet through
 // distributed shared memory.  First all rows' maximum and sum of exponentials in 32 bits (or their largest logit), one read
@@ -84,9 +84,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// (largest value, lowest index among equals)
+// (largest value, lowest index among equals; a NaN is larger than any number, as for the greedy sampler)
 __device__ __forceinline__ void better(float& v, int& i, float w, int k) {
-    if (w > v || (w == v && k < i)) {
+    const bool number = v == v;
+    if (w != w ? number || k < i : number && (w > v || (w == v && k < i))) {
         v = w;
         i = k;
     }
@@ -224,10 +225,11 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, AHEAD_R
         }
         // the warp's lanes
         const float own = top;
-        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(own));
         if (greedy) {
-            index = (int)__reduce_min_sync(0xffffffffu, (unsigned)(own == top ? index : 0x7fffffff));
+            asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(own));
+            index = (int)__reduce_min_sync(0xffffffffu, (unsigned)(own == top || own != own ? index : 0x7fffffff));
         } else {
+            asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(own));
             const float ref = top == -INFINITY ? 0.0f : top;
             sum *= exp2_fast((own - ref) * scale);
 #pragma unroll

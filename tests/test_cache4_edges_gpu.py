@@ -1,0 +1,55 @@
+"""Calls of the 4-bit cache, step tables and verification at the edges of what they take, against the plain statement in
+64 bits."""
+import math
+
+import pytest
+import torch
+
+import plain_cache4 as plain
+
+pytestmark = pytest.mark.gpu
+CUDA = "cuda"
+
+
+def _ops():
+    from pretrained_rstr_b200.csrc import ops
+    return ops
+
+
+def _status():
+    return torch.zeros(4, dtype=torch.int32, device=CUDA)
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32, device=CUDA)
+
+
+def _verify(logits, starts, drafted, uniforms, temps, probs=None):
+    ops = _ops()
+    rows = logits.shape[0]
+    tokens, accepted, status = _ints([9] * rows), _ints([9] * len(temps)), _status()
+    ops.verify_drafts(tokens, accepted, logits.to(CUDA), _ints(starts), _ints(drafted), uniforms.to(CUDA),
+                      torch.tensor(temps, dtype=torch.float32, device=CUDA), status,
+                      draft_probs=None if probs is None else probs.to(CUDA))
+    return (tokens.tolist(), accepted.tolist()), status.tolist()
+
+
+# ------------------------------------------------------------------------------------ verification
+@pytest.mark.parametrize("requests", [1, 40])
+@pytest.mark.parametrize("vocab,places", [(40, [7]), (700, [699, 0]), (50257, [50000, 33001]), (50257, [6284])])
+@pytest.mark.parametrize("follows", [False, True])
+def test_a_nan_wins_a_greedy_row_and_is_reported(requests, vocab, places, follows):
+    """As in the framework's greedy sampler: a NaN among a row's logits wins over every number, the lowest one over other
+    NaN, and the row is reported, whether the draft had that token or the largest number's."""
+    g = torch.Generator().manual_seed(vocab + len(places))
+    logits = torch.randn(3 * requests, vocab, generator=g)
+    starts = list(range(0, 3 * requests + 1, 3))
+    drafted = logits.argmax(-1).tolist()
+    bad = 3 * (requests - 1) + 1
+    logits[bad, places] = math.nan
+    if follows:
+        drafted[bad] = min(places)
+    want = plain.verify(logits, starts, drafted, torch.zeros(3 * requests, 2).tolist(), [0.0] * requests)
+    got, status = _verify(logits, starts, drafted, torch.zeros(3 * requests, 2), [0.0] * requests)
+    assert got == want and got[0][bad] == min(places)
+    assert status[:3] == [7, bad, requests - 1]
