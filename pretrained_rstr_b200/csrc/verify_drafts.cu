@@ -12,7 +12,8 @@
 //
 // One launch; a cluster of eight CTAs takes a request, each an eighth of the vocabulary, and they meet through
 // distributed shared memory.  First all rows' maximum and sum of exponentials in 32 bits (or their largest logit), one read
-// of the logits from memory, which is what bounds it: 64 requests of 5 rows of 50,257 are 64 MB.  Then the one row that is
+// of the logits from memory, which is what bounds it: 64 requests of 5 rows of 50,257 are 64 MB.  That decides who stays, but
+// for a u q next to its p, where the row's sum is taken again in 64 bits.  Then the one row that is
 // drawn from, in 64 bits: the border between two tokens moves by the error of a running sum over the whole vocabulary, and
 // in 32 bits one draw in some hundred would fall on the other side.  The row comes from the L2, where the first pass left
 // it; its exponentials (exp64: 20 operations of 64 bits) are taken once and kept in shared memory where they fit.
@@ -77,8 +78,7 @@ __device__ __forceinline__ double peer_d(const double* p, int rank) {
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
-// 2^x by the hardware approximation (relative error about 2^-22): a sum of many such terms is off by far less than the
-// 2^-24 that a uniform number of 32 bits can tell apart.
+// 2^x by the hardware approximation (relative error about 2^-22)
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -260,10 +260,33 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, AHEAD_R
     }
     cluster_sync_all();
 
+    // the CTA's sum, then all CTAs'
+    int turn = 1;
+    auto meet = [&](double v) -> double {
+        turn ^= 1;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == 0) s.part[turn][warp] = v;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            double a = 0.0;
+            for (int w = 0; w < WARPS; ++w) a += s.part[turn][w];
+            s.total[turn] = a;
+        }
+        cluster_sync_all();
+        double all = 0.0;
+        for (int c = 0; c < PARTS; ++c) all += peer_d(&s.total[turn], c);
+        return all;
+    };
     // -------------------------------- who stays: lane i looks at row i, every warp by itself
     float top = -INFINITY;
     int best = 0x7fffffff;
-    bool stays = false;
+    bool stays = false, unsure = false;
+    const double inverse = 1.0 / (double)t;
+    // What the sum in 32 bits may be off by, of itself.  An exponent is off by 2^-23 of itself (the scale's rounding, the
+    // product's), and a term of exponent -x weighs 2^-x, so a whole row of them by less than 32 x 2^-23; the exponential by
+    // 2^-22, a sum of n terms one after the other by n 2^-24.  Twice that and more is called next to the border.
+    const double doubt = (64 + each / THREADS) * 2.384185791015625e-07;
     if (lane < rows) {
         float part[PARTS], sum = 0.0f;
 #pragma unroll
@@ -289,11 +312,31 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, AHEAD_R
             } else {
                 const double mine = exp64(((double)p.logits[(long)(r0 + lane) * p.logits_stride + x] - (double)ref) / (double)t);
                 const double theirs = p.draft_probs ? (double)p.draft_probs[(long)(r0 + lane) * p.probs_stride + x] : 1.0;
-                stays = (double)p.uniforms[2 * (r0 + lane)] * theirs * (double)sum < mine;
+                const double bar = (double)p.uniforms[2 * (r0 + lane)] * theirs * (double)sum;
+                stays = bar < mine;
+                unsure = fabs(bar - mine) < doubt * mine;
             }
         }
     }
-    const int kept = __ffs(~__ballot_sync(0xffffffffu, stays)) - 1;       // (row rows - 1 never stays)
+    int kept = __ffs(~__ballot_sync(0xffffffffu, stays)) - 1;             // (row rows - 1 never stays)
+    // Next to the border the row's sum is taken again, in 64 bits (one row in some ten thousand; all CTAs come to the same
+    // answers, since they added the same numbers in the same order).
+    unsigned open = __ballot_sync(0xffffffffu, unsure);
+    while (open != 0 && __ffs(open) - 1 <= kept) {
+        const int r = __ffs(open) - 1;
+        open &= open - 1;
+        const float* x = p.logits + (long)(r0 + r) * p.logits_stride;
+        const double ref = (double)__shfl_sync(0xffffffffu, top, r);
+        double v = 0.0;
+        for (int i = lo + threadIdx.x; i < hi; i += THREADS) v += exp64(((double)x[i] - ref) * inverse);
+        const double whole = meet(v);
+        if (lane == r) {
+            const int token = p.drafted[r0 + r];
+            const double theirs = p.draft_probs ? (double)p.draft_probs[(long)(r0 + r) * p.probs_stride + token] : 1.0;
+            stays = (double)p.uniforms[2 * (r0 + r)] * theirs * whole < exp64(((double)x[token] - ref) * inverse);
+        }
+        kept = __ffs(~__ballot_sync(0xffffffffu, stays)) - 1;
+    }
     const int row = r0 + kept;
     const bool refused = kept + 1 < rows;
     int chosen = __shfl_sync(0xffffffffu, best, kept);
@@ -305,27 +348,8 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, AHEAD_R
         const float* x = p.logits + (long)row * p.logits_stride;
         const float* q = refused && p.draft_probs ? p.draft_probs + (long)row * p.probs_stride : nullptr;
         const int gone = refused && !p.draft_probs ? p.drafted[row] : -1;
-        const double inverse = 1.0 / (double)t;
         const int run = (hi - lo + WARPS - 1) / WARPS;
         const int w0 = min(lo + warp * run, hi), w1 = min(w0 + run, hi);
-        // the CTA's sum, then all CTAs'
-        int turn = 1;
-        auto meet = [&](double v) -> double {
-            turn ^= 1;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            if (lane == 0) s.part[turn][warp] = v;
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                double a = 0.0;
-                for (int w = 0; w < WARPS; ++w) a += s.part[turn][w];
-                s.total[turn] = a;
-            }
-            cluster_sync_all();
-            double all = 0.0;
-            for (int c = 0; c < PARTS; ++c) all += peer_d(&s.total[turn], c);
-            return all;
-        };
         const bool keep = each <= KEPT;
         if (q != nullptr)                                                 // (wanted once the sum below is known)
             for (int i = lo + 32 * threadIdx.x; i < hi; i += 32 * THREADS)

@@ -53,3 +53,29 @@ def test_a_nan_wins_a_greedy_row_and_is_reported(requests, vocab, places, follow
     got, status = _verify(logits, starts, drafted, torch.zeros(3 * requests, 2), [0.0] * requests)
     assert got == want and got[0][bad] == min(places)
     assert status[:3] == [7, bad, requests - 1]
+
+
+@pytest.mark.parametrize("certain", [True, False])
+@pytest.mark.parametrize("requests,vocab,t", [(30, 50257, 1.1), (64, 50257, 0.8), (30, 50257, 0.3), (64, 5003, 1.3), (20, 131072, 1.0)])
+def test_numbers_next_to_the_border_decide_by_it(requests, vocab, t, certain):
+    """u * q < p for the float32 numbers u right below and right above p / q: the border itself in 64 bits."""
+    g = torch.Generator().manual_seed(vocab)
+    logits = 2.5 * torch.randn(2 * requests, vocab, generator=g)
+    t = float(torch.tensor(t))
+    p = torch.softmax(logits.double() / t, -1)
+    drafted = torch.multinomial(p, 1, generator=g)[:, 0]
+    rows = torch.arange(2 * requests)
+    mine = p[rows, drafted]
+    q = torch.zeros(2 * requests, vocab)
+    q[rows, drafted] = 1.0 if certain else (mine.float() * (1.0 + torch.rand(2 * requests, generator=g)))
+    border = mine / q[rows, drafted].double()
+    below = border.float()
+    below = torch.where(below.double() >= border, torch.nextafter(below, torch.zeros(1)), below)
+    above = torch.nextafter(below, torch.ones(1))
+    starts = list(range(0, 2 * requests + 1, 2))
+    for u, stays in ((below, 1), (above, 0)):
+        assert bool(((u.double() * q[rows, drafted].double() < mine) == bool(stays)).all())
+        uniforms = torch.stack([u, torch.full_like(u, 0.5)], 1)
+        (tokens, accepted), status = _verify(logits, starts, drafted.tolist(), uniforms, [t] * requests, None if certain else q)
+        assert status == [0] * 4
+        assert accepted == [stays] * requests
