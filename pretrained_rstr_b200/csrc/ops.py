@@ -2940,7 +2940,8 @@ def verify_drafts(tokens, accepted, logits, row_start, drafted, uniforms, temper
     Request b has the rows ``row_start[b]`` to ``row_start[b + 1] - 1`` of ``logits`` float32 [rows, vocabulary]: one
     more than it drafted tokens (at most ``VERIFY_DRAFTS_MAX_TOKENS``); row i of a request is the target's answer
     behind its i-th drafted token, and ``drafted[row]`` the token that the draft put there (of a request's last row:
-    not read).  ``temperature`` float32 [requests]: the target's probabilities are softmax(logits / temperature); 0 or
+    not read).  ``temperature`` float32 [requests]: the target's probabilities are softmax(logits / temperature), for
+    an infinite one all tokens of finite logits alike; 0 or
     less is greedy: the largest logit, the lowest index among equals, a NaN before all numbers (and in the status word).
     ``draft_probs`` float32 [rows, vocabulary]: what the draft drew each token from (None: the draft
     was sure of its tokens).  ``uniforms`` float32 [rows, 2], in [0, 1): the first decides whether the row's token

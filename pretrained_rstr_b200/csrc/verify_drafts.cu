@@ -136,7 +136,10 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, AHEAD_R
     }
     const float t = p.temperature[req];
     const bool greedy = !(t > 0.0f);
-    const float scale = greedy ? 1.0f : 1.4426950408889634f / t;
+    // (of temperatures whose scale is 0 or no number in 32 bits the products below are none either: it stops before that, and
+    // the sums of such rows are looked at in 64 bits)
+    const float scale = greedy ? 1.0f : fminf(fmaxf(1.4426950408889634f / t, 1e-37f), 1e37f);
+    const bool extreme = !(t > 1e-30f && t < 1e30f);
     // this CTA's tokens, and each warp's run of them
     const int each = (p.vocab + PARTS - 1) / PARTS;
     const int lo = min(rank * each, p.vocab), hi = min(lo + each, p.vocab);
@@ -314,7 +317,7 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, AHEAD_R
                 const double theirs = p.draft_probs ? (double)p.draft_probs[(long)(r0 + lane) * p.probs_stride + x] : 1.0;
                 const double bar = (double)p.uniforms[2 * (r0 + lane)] * theirs * (double)sum;
                 stays = bar < mine;
-                unsure = fabs(bar - mine) < doubt * mine;
+                unsure = extreme || fabs(bar - mine) < doubt * mine;
             }
         }
     }

@@ -79,3 +79,20 @@ def test_numbers_next_to_the_border_decide_by_it(requests, vocab, t, certain):
         (tokens, accepted), status = _verify(logits, starts, drafted.tolist(), uniforms, [t] * requests, None if certain else q)
         assert status == [0] * 4
         assert accepted == [stays] * requests
+
+
+@pytest.mark.parametrize("t", [math.inf, 1e38, 1e-42, 1e-38])
+@pytest.mark.parametrize("requests", [3, 40])
+def test_the_largest_and_the_smallest_temperatures(requests, t):
+    """At an endless temperature all tokens are as likely, at one next to 0 only the largest logits are."""
+    g = torch.Generator().manual_seed(5)
+    logits = torch.round(2 * torch.randn(3 * requests, 501, generator=g))
+    starts = list(range(0, 3 * requests + 1, 3))
+    drafted = logits.argmax(-1)
+    drafted[::2] = torch.randint(501, drafted[::2].shape, generator=g)
+    uniforms = torch.rand(3 * requests, 2, generator=g)
+    uniforms[::4, 0] *= 0.003
+    t = float(torch.tensor(t, dtype=torch.float32))
+    want = plain.verify(logits, starts, drafted.tolist(), uniforms.tolist(), [t] * requests)
+    got, status = _verify(logits, starts, drafted.tolist(), uniforms, [t] * requests)
+    assert status == [0] * 4 and got == want
