@@ -2950,7 +2950,9 @@ def verify_drafts(tokens, accepted, logits, row_start, drafted, uniforms, temper
     drafted token, the lowest index at which the running sum passes the number's share of the whole.
 
     Written: ``accepted[b]``: drafted tokens that stay; ``tokens`` int32 [rows]: they and the token behind them, -1 in
-    the request's rows beyond.  Neither shares memory with another tensor of the call."""
+    the request's rows beyond.  A request of no rows, of more than ``VERIFY_DRAFTS_MAX_TOKENS`` + 1 or of rows outside
+    ``logits`` is in the status word: none accepted, -1 in all of its rows; where they lie outside, no row is written.
+    Neither shares memory with another tensor of the call."""
     what = "verify_drafts"
     device = logits.get_device()
     if device < 0 or tokens.get_device() != device or accepted.get_device() != device or \

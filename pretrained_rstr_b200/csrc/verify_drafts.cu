@@ -132,6 +132,9 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, AHEAD_R
             prb_set_status(p.status, PRB_S_ROW_RANGE, r0, r1, p.n_rows);
             p.accepted[req] = 0;
         }
+        // (what an earlier step left in its rows is not an answer; a range that leaves the tensor names no rows)
+        if (r0 >= 0 && r1 <= p.n_rows)
+            for (int r = r0 + rank * THREADS + (int)threadIdx.x; r < r1; r += PARTS * THREADS) p.tokens[r] = -1;
         return;
     }
     const float t = p.temperature[req];

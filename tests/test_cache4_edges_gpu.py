@@ -96,3 +96,14 @@ def test_the_largest_and_the_smallest_temperatures(requests, t):
     want = plain.verify(logits, starts, drafted.tolist(), uniforms.tolist(), [t] * requests)
     got, status = _verify(logits, starts, drafted.tolist(), uniforms, [t] * requests)
     assert status == [0] * 4 and got == want
+
+
+@pytest.mark.parametrize("rows", [33, 40, 200])
+def test_a_request_of_too_many_rows_has_no_tokens(rows):
+    """Refused and recorded; its rows say so (-1) instead of what an earlier step left there, its neighbours are as ever."""
+    g = torch.Generator().manual_seed(rows)
+    logits = torch.randn(rows + 4, 50, generator=g)
+    drafted = logits.argmax(-1).tolist()
+    (tokens, accepted), status = _verify(logits, [0, 2, 2 + rows, rows + 4], drafted, torch.zeros(rows + 4, 2), [0.0] * 3)
+    assert status[0] == 6 and accepted == [1, 0, 1]
+    assert tokens == drafted[:2] + [-1] * rows + drafted[-2:]
