@@ -482,6 +482,11 @@ attention_4bit_kernel(const Args p) {
                     s[c][z][e + EN] = sum[z][e + 2];
                 }
         }
+        // (which weights are 0 because their key is masked: a weight that is 0 because e^x has no smaller number still makes NaN
+        // of a value that is none)
+        uint32_t hidden = 0;
+        static_assert(NC * QN * 2 * EN <= 32, "a bit a score");
+        auto is_hidden = [&](int c, int z, int e) -> bool { return (hidden >> ((c * QN + z) * 2 * EN + e)) & 1u; };
         if (masked) {
 #pragma unroll
             for (int c = 0; c < NC; ++c)
@@ -490,7 +495,10 @@ attention_4bit_kernel(const Args p) {
 #pragma unroll
                     for (int e = 0; e < 2 * EN; ++e) {
                         const int key = key0 + c * 16 + n + 8 * (e / EN), at = pos[z][e % EN];
-                        if (key > at || (p.window > 0 && key <= at - p.window)) s[c][z][e] = -INFINITY;
+                        if (key > at || (p.window > 0 && key <= at - p.window)) {
+                            s[c][z][e] = -INFINITY;
+                            hidden |= 1u << ((c * QN + z) * 2 * EN + e);
+                        }
                     }
         }
         // ---- maximum, exponentials
@@ -574,8 +582,8 @@ attention_4bit_kernel(const Args p) {
 #pragma unroll
                         for (int g = 0; g < NG; ++g) {
                             float y = 0.0f;
-                            if (s[c][z][e] != 0.0f) y += s[c][z][e] * __uint_as_float(pr[0][g] & 0xffff0000u);
-                            if (s[c][z][e + EN] != 0.0f) y += s[c][z][e + EN] * __uint_as_float(pr[1][g] & 0xffff0000u);
+                            if (!is_hidden(c, z, e)) y += s[c][z][e] * __uint_as_float(pr[0][g] & 0xffff0000u);
+                            if (!is_hidden(c, z, e + EN)) y += s[c][z][e + EN] * __uint_as_float(pr[1][g] & 0xffff0000u);
 #pragma unroll
                             for (int o2 = 4; o2 < 32; o2 <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o2);
                             if (n == g) mid[z][e] += y;
@@ -605,8 +613,8 @@ attention_4bit_kernel(const Args p) {
                         x[e] = s[c][z][e] * step0;
                         x[e + EN] = s[c][z][e + EN] * step1;
                         if (masked) {
-                            if (s[c][z][e] == 0.0f) x[e] = 0.0f;
-                            if (s[c][z][e + EN] == 0.0f) x[e + EN] = 0.0f;
+                            if (is_hidden(c, z, e)) x[e] = 0.0f;
+                            if (is_hidden(c, z, e + EN)) x[e + EN] = 0.0f;
                         }
                     }
                     uint32_t b0[PIECES], b1[PIECES];

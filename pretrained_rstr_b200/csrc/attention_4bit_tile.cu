@@ -594,11 +594,11 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
             for (int z = 0; z < p.parts; ++z) top = fmaxf(top, lds_cluster(cluster_addr(smem_u32(state_m + r), z)));
 #pragma unroll
             for (int z = 0; z < MAX_PARTS; ++z) {
-                weight[z] = 0.0f;
+                weight[z] = -1.0f;                                 // (no keys of the row's: there may be no results)
                 if (z < p.parts) {
                     const float mz = lds_cluster(cluster_addr(smem_u32(state_m + r), z));
-                    weight[z] = mz == -INFINITY ? 0.0f : exp2_fast(mz - top);
-                    sum += weight[z] * lds_cluster(cluster_addr(smem_u32(state_l + r), z));
+                    if (mz != -INFINITY) weight[z] = exp2_fast(mz - top);
+                    sum += fmaxf(weight[z], 0.0f) * lds_cluster(cluster_addr(smem_u32(state_l + r), z));
                 }
             }
             const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
                 float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int z = 0; z < MAX_PARTS; ++z)
-                    if (z < p.parts && weight[z] > 0.0f) {
+                    if (z < p.parts && weight[z] >= 0.0f) {        // (0 times NaN goes on)
                         const uint32_t at = cluster_addr(smem_u32(state + (size_t)ch * QT + r), z);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) x[i] = fmaf(weight[z], lds_cluster(at + i * QT * 4), x[i]);

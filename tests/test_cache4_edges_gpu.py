@@ -107,3 +107,50 @@ def test_a_request_of_too_many_rows_has_no_tokens(rows):
     (tokens, accepted), status = _verify(logits, [0, 2, 2 + rows, rows + 4], drafted, torch.zeros(rows + 4, 2), [0.0] * 3)
     assert status[0] == 6 and accepted == [1, 0, 1]
     assert tokens == drafted[:2] + [-1] * rows + drafted[-2:]
+
+
+# ------------------------------------------------------------------------------------ attention
+def _cached(k, v, page):
+    n, kv, d = k.shape
+    pages = -(-n // page)
+
+    def one(x):
+        full = torch.zeros(pages * page, kv, d)
+        full[:n] = x
+        return plain.pack(*plain.quantize(full.view(pages, page, kv, d).transpose(1, 2))).to(CUDA)
+    return one(k), one(v), _ints([list(range(pages))])
+
+
+def _attend(k, v, q, held, page, scale, parts=0, window=None, status_word=0):
+    """The tokens behind ``held`` positions of one request, in tiles of up to 128 rows."""
+    ops = _ops()
+    total, kv, d = k.shape
+    new, heads = total - held, q.shape[1] // d
+    kt, vt, table = _cached(k, v, page)
+    most = max(1, 128 * kv // heads)
+    tiles = plain.tiles_of([new], most)
+    out, status = torch.full((new, heads * d), 3.0, dtype=q.dtype, device=CUDA), _status()
+    ops.attention_4bit(out, q.to(CUDA), kt, vt, table, _ints(list(range(held, total))), *(_ints(list(x)) for x in zip(*tiles)),
+                       min(new, most), heads, d, page, scale, window, total, status, parts=parts)
+    assert status.tolist()[0] == status_word
+    return out.float().cpu().view(new, heads, d)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv,d,page", [(2, 2, 64, 64), (4, 1, 128, 64), (2, 1, 96, 32), (3, 3, 16, 16)])
+@pytest.mark.parametrize("held,new,parts", [(99, 1, 1), (99, 1, 0), (299, 1, 4), (200, 40, 1), (200, 40, 4), (200, 5, 2), (200, 12, 1)])
+@pytest.mark.parametrize("bad", [3, 98])
+def test_a_value_that_is_no_number_under_a_weight_of_nearly_nothing(bad, held, new, parts, heads, kv, d, page, dtype):
+    """Nearly nothing times NaN is NaN, in whichever stage or part of the keys the value lies."""
+    g = torch.Generator().manual_seed(new)
+    total = held + new
+    k, v = 0.1 * torch.randn(total, kv, d, generator=g), torch.randn(total, kv, d, generator=g)
+    q = 4.0 + 0.1 * torch.randn(new, heads * d, generator=g)
+    k[held - 5 if held > 104 else 90] = 6.0                               # e^-300 and less for all the others
+    want = _attend(k, v, q.to(dtype), held, page, 1.0, parts)
+    v[bad, kv - 1, d - 1] = math.nan
+    got = _attend(k, v, q.to(dtype), held, page, 1.0, parts)
+    nan = torch.zeros(new, heads, d, dtype=torch.bool)
+    nan[:, heads - heads // kv:, (d - 1) // 32 * 32:] = True
+    assert torch.equal(torch.isnan(got), nan)
+    assert torch.equal(got[~nan], want[~nan])
