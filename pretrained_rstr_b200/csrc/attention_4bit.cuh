@@ -8,7 +8,8 @@
 // The codes less 8 are whole numbers from -8 to 7, exact in bfloat16, so the cache is never turned into rounded
 // numbers: the products run on the matrix units (mma.sync, 16 x 8 x 16) with the codes as one operand, and the
 // steps and middles join in 32 bits.  bfloat16 queries are exact too, and p * step is the one rounding (2^-8,
-// as probabilities are rounded before any such product).  float32 queries, and then p * step, go as the sum of
+// as probabilities are rounded before any such product); p * middle is summed in 32 bits, since a group's middle may be many
+// of its steps.  float32 queries, and then p * step, go as the sum of
 // three bfloat16 numbers (24 bits), which makes three products of 32-bit exactness.
 //
 // Keys and values are the left operand (16 keys x 16 channels, 16 channels x 16 keys), queries and probabilities the
@@ -394,8 +395,8 @@ attention_4bit_kernel(const Args p) {
     }
 
     // results [rows][group][16 of its channels]: channels (2 i, 2 i + 1 of the thread's four) x rows (2 j, 2 j + 1); sums of
-    // p * middle of group n
-    float o[QN][NG][2][4], mid[QN][4];
+    // p * middle over the lane's keys, of rows 2 j, 2 j + 1
+    float o[QN][NG][2][4], mid[QN][EN][NG];
     float m[QN][EN], l[QN][EN];
 #pragma unroll
     for (int z = 0; z < QN; ++z) {
@@ -403,13 +404,13 @@ attention_4bit_kernel(const Args p) {
         for (int e = 0; e < EN; ++e) {
             m[z][e] = -INFINITY;
             l[z][e] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) mid[z][e][g] = 0.0f;
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            mid[z][i] = 0.0f;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int g = 0; g < NG; ++g) o[z][g][0][i] = o[z][g][1][i] = 0.0f;
-        }
     }
     const float sl2 = p.scale * 1.4426950408889634f;          // scores are handled in log2 units
     // (the short last group's rows are 8 bytes apart; its words 2 and 3 do not exist: words 0 and 1 stand in, against
@@ -535,9 +536,9 @@ attention_4bit_kernel(const Args p) {
                 for (int i = 0; i < 4; ++i) {
                     if ((i & 1) >= EN) continue;
                     const float by = alpha[z][(i & 1) % EN];
-                    mid[z][i] *= by;
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
+                        if (i < 2) mid[z][i % EN][g] *= by;
                         o[z][g][0][i] *= by;
                         o[z][g][1][i] *= by;
                     }
@@ -552,42 +553,18 @@ attention_4bit_kernel(const Args p) {
             uint32_t pr[2][NG];
             load_params<NG>(par + n * NG * 4, pr[0]);
             load_params<NG>(par + (n + 8) * NG * 4, pr[1]);
-            if (!masked) {
-                // p * middle: rows of the left operand are groups (n, those beyond the last stand in for themselves)
-                const uint8_t* col = par + (NG == 1 ? 0 : NG == 2 ? (n & 1) : NG == 4 ? (n & 3) : min(n, 2)) * 4 + 2;
-                auto middle = [&](int key) -> uint32_t { return *reinterpret_cast<const uint16_t*>(col + key * NG * 4); };
-                const uint32_t a0 = middle(j) | (middle(j + 8) << 16);
-                const uint32_t a1 = middle(j + 4) | (middle(j + 12) << 16);
+            // p * middle, in 32 bits: a lane's keys by themselves, all lanes' in the end.  (A masked key's middle may be
+            // anything, NaN too.)
 #pragma unroll
-                for (int z = 0; z < QN; ++z) {
-                    uint32_t b0[PIECES], b1[PIECES];
-                    as_operand<EN, PIECES>(s[c][z], lane, b0, b1);
-                    if (EXACT) {
-                        float part[4];
-                        mma0(part, a0, 0u, a1, 0u, b0[PIECES - 1], b1[PIECES - 1]);
-#pragma unroll
-                        for (int k = PIECES - 2; k >= 0; --k) mma(part, a0, 0u, a1, 0u, b0[k], b1[k]);
-#pragma unroll
-                        for (int e = 0; e < EN; ++e) mid[z][e] += part[e];
-                    } else {
-                        mma(mid[z], a0, 0u, a1, 0u, b0[0], b1[0]);
-                    }
-                }
-            } else {
-                // A masked key's middle may be anything, NaN too, which a product would spread over all rows.
+            for (int g = 0; g < NG; ++g) {
+                const float middle0 = __uint_as_float(pr[0][g] & 0xffff0000u), middle1 = __uint_as_float(pr[1][g] & 0xffff0000u);
 #pragma unroll
                 for (int z = 0; z < QN; ++z)
 #pragma unroll
-                    for (int e = 0; e < EN; ++e)
-#pragma unroll
-                        for (int g = 0; g < NG; ++g) {
-                            float y = 0.0f;
-                            if (!is_hidden(c, z, e)) y += s[c][z][e] * __uint_as_float(pr[0][g] & 0xffff0000u);
-                            if (!is_hidden(c, z, e + EN)) y += s[c][z][e + EN] * __uint_as_float(pr[1][g] & 0xffff0000u);
-#pragma unroll
-                            for (int o2 = 4; o2 < 32; o2 <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o2);
-                            if (n == g) mid[z][e] += y;
-                        }
+                    for (int e = 0; e < EN; ++e) {
+                        if (!masked || !is_hidden(c, z, e)) mid[z][e][g] = fmaf(s[c][z][e], middle0, mid[z][e][g]);
+                        if (!masked || !is_hidden(c, z, e + EN)) mid[z][e][g] = fmaf(s[c][z][e + EN], middle1, mid[z][e][g]);
+                    }
             }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
@@ -695,7 +672,9 @@ attention_4bit_kernel(const Args p) {
             }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const float y = __shfl_sync(0xffffffffu, mid[z][e], g * 4 + j);
+                float y = mid[z][e][g];
+#pragma unroll
+                for (int o2 = 4; o2 < 32; o2 <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o2);
                 float* at = st + g * 32 + 8 * (n & 3) + 4 * (n >> 2);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {

@@ -154,3 +154,44 @@ def test_a_value_that_is_no_number_under_a_weight_of_nearly_nothing(bad, held, n
     nan[:, heads - heads // kv:, (d - 1) // 32 * 32:] = True
     assert torch.equal(torch.isnan(got), nan)
     assert torch.equal(got[~nan], want[~nan])
+
+
+@pytest.mark.parametrize("heads,kv,d,page", [(2, 2, 64, 64), (12, 12, 64, 64), (4, 1, 128, 64), (2, 1, 96, 32), (3, 3, 16, 16)])
+@pytest.mark.parametrize("held,new", [(99, 1), (1000, 1), (300, 5), (500, 12), (63, 32)])
+def test_equal_values_come_back_as_they_are(held, new, heads, kv, d, page):
+    """Values that are all one number: whatever the weights are, they add up to one, so the result is that number.  A weight
+    rounded to bfloat16 (2^-8 of itself) would show; in 32 bits what is lost is far below half a step of the result.
+    (Where the number's step is 0 there is nothing that p * step rounds.)"""
+    if new * heads > 32 * kv:
+        pytest.skip("a portion of a prompt: its kernel rounds weights to bfloat16")
+    g = torch.Generator().manual_seed(held + new)
+    total = held + new
+    # scores of 0 and of ln(0.50195...): weights 1 and 0.5 + 2^-9, which lies half way between two bfloat16 numbers
+    k = torch.zeros(total, kv, d)
+    k[torch.rand(total, generator=g) < 0.9] = -1.0
+    q = torch.full((new, heads * d), 0.5)
+    scale = -math.log(0.5 + 2.0 ** -9 * 1.02) / (0.5 * d)
+    for number in (8.0, -0.0078125, 1.5):
+        out = _attend(k, torch.full((total, kv, d), number), q.to(torch.bfloat16), held, page, scale)
+        assert bool((out == number).all()), float((out - number).abs().max() / abs(number))
+
+
+@pytest.mark.parametrize("heads,kv,d,page,held,new,window", [
+    (12, 12, 64, 64, 999, 1, None), (2, 2, 64, 64, 300, 5, None), (4, 1, 128, 64, 700, 6, None), (2, 1, 96, 32, 90, 12, None),
+    (3, 3, 16, 16, 200, 30, None), (4, 4, 64, 64, 800, 1, 500), (1, 1, 64, 64, 3000, 8, 2000)])
+def test_weights_meet_middles_unrounded(heads, kv, d, page, held, new, window):
+    """Channels with an offset, as keys and values of real models have: a result is off by half a step of its own (2^-8), of
+    every weight times its step (2^-8), and by what sums in 32 bits lose: no weight is rounded before it meets an offset."""
+    g = torch.Generator().manual_seed(held)
+    total = held + new
+    k = torch.randn(total, kv, d, generator=g)
+    v = 0.3 * torch.randn(total, kv, d, generator=g) + 5.0 * torch.randn(kv, d, generator=g).sign()
+    q = torch.randn(new, heads * d, generator=g).to(torch.bfloat16)
+    scale = 1.0 / math.sqrt(d)
+    got = _attend(k, v, q, held, page, scale, window=window).flatten(1)
+    kt, vt, table = _cached(k, v, page)
+    ref, (a, b, e) = plain.attention(q, kt.cpu(), vt.cpu(), table.tolist(), list(range(held, total)), [0] * new, heads, d, page,
+                                     scale, window)
+    wide = 2 * (1.01 * e + 2.0 ** -21 + 2.0 ** -17) + (total + 16) * 2.0 ** -23
+    worst = float(((got.double() - ref).abs() / (1.01 * 2.0 ** -8 * (ref.abs() + a) + wide * b)).max())
+    assert worst <= 1.0, f"{worst:.2f} of the bound"
