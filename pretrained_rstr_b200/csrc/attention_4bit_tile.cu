@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
             const uint8_t* src = raw + rs * 2 * RAW + KIND * RAW;
             const uint32_t stage = smem_u32(ring + (size_t)st * STAGE) + KIND * 2 * ND * TILE;
             constexpr int TASKS = 8 * NG / DEQUANT;
-            uint32_t word[TASKS], pair[TASKS];
+            uint32_t word[TASKS], pair[TASKS], large = 0u;
 #pragma unroll
             for (int i = 0; i < TASKS; ++i) {
                 const int task = (t >> 5) + i * DEQUANT, g = task >> 3, key = (task & 7) * 8 + key8;
@@ -470,6 +470,8 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
                     word[i] = *reinterpret_cast<const uint32_t*>(src + g * KB * 16 + key * (head_dim - g * 32 >= 32 ? 16 : 8) + w * 4);
                     pair[i] = *reinterpret_cast<const uint32_t*>(src + KB * (head_dim / 2) + (key * ng + g) * 4);
                 }
+                // (bits 15 and 31: a step or a middle of 2^124 or more)
+                if (KIND == 1) large |= (pair[i] & 0x7fff7fffu) + 0x02000200u;
             }
             // (channels i and i + 4 of a word's 8 lie together, as one shift and one mask take them from it: the queries are
             // laid out alike, and the results' channels are put right when they are stored)
@@ -496,6 +498,15 @@ __global__ void __launch_bounds__(THREADS, ND == 1 ? 2 : 1) attention_4bit_tile_
                                                          __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), off),
                                                          *reinterpret_cast<const __nv_bfloat162*>(&middle));
                         hi[e] = *reinterpret_cast<const uint32_t*>(&v);
+                    }
+                    // A code may stand for more than the largest bfloat16 number: that one then (1 % off at most), since an
+                    // infinity would make NaN of the rows that do not see the key.
+                    if (large & 0x80008000u) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if ((hi[e] & 0x7fffu) == 0x7f80u) hi[e] -= 1u;
+                            if ((hi[e] & 0x7fff0000u) == 0x7f800000u) hi[e] -= 0x10000u;
+                        }
                     }
                     st_shared_v4(at, hi[0], hi[1], hi[2], hi[3]);
                 } else {
