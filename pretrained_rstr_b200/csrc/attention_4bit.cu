@@ -45,7 +45,9 @@ PRB_API int prb_attention_4bit(void* out, long out_stride, const void* q, long q
     if (heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || tile_most <= 0 || !cache4::takes(head_dim, page_size) ||
         max_pages <= 0 || num_pages <= 0 || n_requests <= 0 || (long)max_pages * page_size > 0x7fffffffL)
         return PRB_E_SIZE;
-    if (window < 0 || max_context <= 0 || parts < 0 || parts > attn4::MAX_PARTS) return PRB_E_ARG;
+    if (window < 0 || max_context <= 0 || parts < 0 || parts > attn4::MAX_PARTS ||
+        !(scale > 0.0f && scale <= 1e37f))                   // (scores are masked and compared before they are scaled)
+        return PRB_E_ARG;
     if ((uintptr_t)k_tiles % 16 != 0 || (uintptr_t)v_tiles % 16 != 0) return PRB_E_ALIGN;
     if (dtype != PRB_F32 && dtype != PRB_BF16) return PRB_E_DTYPE;
     const int size = dtype == PRB_F32 ? 4 : 2, hpg = heads / kv_heads;

@@ -2831,8 +2831,8 @@ def attention_4bit(out, q, k_tiles, v_tiles, block_table, positions, tile_req, t
     tile_rows[i] - 1``, neighbours of request ``tile_req[i]`` (a row of the block table) at neighbouring positions;
     no tile has more than ``tile_most`` of them, and 128 rows (tokens times the heads that share a key/value head) a
     tile are about what a portion of a prompt should be cut into; a decoded token is a tile of one.  ``tile_count``:
-    int32 on the device, how many of the tiles count (all by default).  ``window``: a token sees its last ``window``
-    positions only.  ``max_context``: the most positions a request holds (the keys are cut into parts by it).
+    int32 on the device, how many of the tiles count (all by default).  ``scale`` (of q . k): above 0, float32 up to 1e37.  ``window``: a
+    token sees its last ``window`` positions only.  ``max_context``: the most positions a request holds (the keys are cut into parts by it).
     ``parts``: CTAs that share a tile's keys (0: the kernel's rule).  Rows of no tile stay as they were."""
     what = "attention_4bit"
     device = q.get_device()
@@ -2850,10 +2850,10 @@ def attention_4bit(out, q, k_tiles, v_tiles, block_table, positions, tile_req, t
         window = 0
     elif window < 1:
         raise KernelArgumentError(f"{what}: a window holds at least the token itself")
-    if tile_most < 1 or max_context < 1 or not 0 <= parts <= ATTENTION_4BIT_MAX_PARTS or not math.isfinite(scale):
+    if tile_most < 1 or max_context < 1 or not 0 <= parts <= ATTENTION_4BIT_MAX_PARTS or not 0.0 < scale < math.inf:
         raise KernelArgumentError(f"{what}: tile_most and max_context are at least 1, parts 0 to "
-                                  f"{ATTENTION_4BIT_MAX_PARTS}, scale is finite; got {tile_most}, {max_context}, {parts}, "
-                                  f"{scale}")
+                                  f"{ATTENTION_4BIT_MAX_PARTS}, scale is finite and above 0; got {tile_most}, "
+                                  f"{max_context}, {parts}, {scale}")
     width = n_heads * head_dim
     q_stride = _matrix4(what, "q", q, 0, width)
     tokens = q.shape[0]

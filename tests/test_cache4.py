@@ -286,3 +286,17 @@ def test_layout_of_caches_in_4_bits():
     with pytest.raises(ValueError, match="no keys and values"):
         _layout(4, [None])
     assert _layout(None, [None]).group_specs == []
+
+
+# ------------------------------------------------------------------------------------ the edges of what the calls take
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.125, -math.inf, math.inf])
+def test_a_scale_that_is_not_above_zero_is_refused(ops, scale):
+    """Scores are masked and compared before they are scaled: a scale below zero would make the masked ones the largest."""
+    with pytest.raises(ops.KernelArgumentError, match="scale"):
+        ops.attention_4bit(**_attention_args(scale=scale))
+
+
+@pytest.mark.parametrize("scale", [1e-60, 1e300, 1e38])
+def test_a_scale_that_32_bits_do_not_hold_is_refused(real_ops, scale):
+    with pytest.raises(real_ops.KernelArgumentError, match="bad argument"):
+        real_ops.attention_4bit(**_attention_args(scale=scale))
