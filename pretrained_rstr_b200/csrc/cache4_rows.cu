@@ -183,9 +183,13 @@ int launch_rows(bool append, RowArgs a, int dtype, cudaStream_t stream) {
         wide = wide && (uintptr_t)a.rows[i] % 16 == 0 && (a.stride[i] * size) % 16 == 0;
     }
     const long pool = a.num_pages * (long)a.heads * cache4::tile_bytes(a.head_dim, a.page_size);
-    if (append ? prb_overlap({a.tiles[0], pool}, {a.tiles[1], pool})
-               : !prb_rows_apart(a.rows[0], a.stride[0] * size, a.rows[1], a.stride[1] * size, a.n_tokens,
-                                 (long)a.heads * a.head_dim * size))
+    const long width = (long)a.heads * a.head_dim * size, word = sizeof(int);
+    const PrbRange keys{a.tiles[0], pool}, values{a.tiles[1], pool}, slots{a.slots, a.n_tokens * word}, status{a.status, 4 * word};
+    const PrbRange k{a.rows[0], prb_span(a.n_tokens, a.stride[0] * size, width)};
+    const PrbRange v{a.rows[1], prb_span(a.n_tokens, a.stride[1] * size, width)};
+    if (append ? !prb_apart({keys, values, status}, {k, v, slots})
+               : !prb_rows_apart(a.rows[0], a.stride[0] * size, a.rows[1], a.stride[1] * size, a.n_tokens, width) ||
+                     !prb_apart({k, status}, {keys, values, slots}) || !prb_apart({v, status}, {keys, values, slots}))
         return PRB_E_OVERLAP;
     a.groups = cache4::groups_of(a.head_dim);
     const int threads_of_token = append ? 2 * a.heads * a.groups * 4 : 2 * a.heads * (a.head_dim / 8);

@@ -2777,7 +2777,7 @@ def kv_append_4bit(k_tiles, v_tiles, k, v, slots, n_tokens: int, head_dim: int, 
     """Round the step's keys and values to 4 bits at their cache slots.  ``k_tiles`` / ``v_tiles``: uint8 [pages,
     kv_heads, ``cache4_tile_bytes(head_dim, page_size)``]; ``k`` / ``v``: [T, kv_heads * head_dim] bfloat16 or float32,
     may be column slices of a wider tensor; ``slots`` int32: page * page_size + place of each token, below zero = none.
-    No two tokens have one slot, and the two tensors of tiles are two.
+    No two tokens have one slot, and neither tensor of tiles shares memory with another tensor of the call.
 
     Of every 32 channels (the last group may be shorter) the cache keeps step = (largest - smallest) / 15 and middle =
     smallest + 8 step in bfloat16 and per channel the nearest of 16 codes; code c reads back as middle + step * (c - 8).
@@ -2801,7 +2801,7 @@ def kv_append_4bit(k_tiles, v_tiles, k, v, slots, n_tokens: int, head_dim: int, 
 def kv_read_4bit(k_out, v_out, k_tiles, v_tiles, slots, n_tokens: int, head_dim: int, page_size: int, status) -> None:
     """What a cache held in 4 bits stands for at ``slots`` (see :func:`kv_append_4bit`): rows of ``k_out`` / ``v_out``
     [T, kv_heads * head_dim], float32 (exact but for a last rounding to 32 bits) or bfloat16.  Rows whose slot is below
-    zero stay as they were."""
+    zero stay as they were.  ``k_out`` and ``v_out`` may be columns of one tensor; else they share memory with nothing."""
     what = "kv_read_4bit"
     device = k_tiles.get_device()
     if device < 0 or v_tiles.get_device() != device or k_out.get_device() != device or v_out.get_device() != device or \

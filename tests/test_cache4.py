@@ -300,3 +300,36 @@ def test_a_scale_that_is_not_above_zero_is_refused(ops, scale):
 def test_a_scale_that_32_bits_do_not_hold_is_refused(real_ops, scale):
     with pytest.raises(real_ops.KernelArgumentError, match="bad argument"):
         real_ops.attention_4bit(**_attention_args(scale=scale))
+
+
+def _over(a, ours, theirs, end):
+    """The arguments with tensor ``ours`` beginning in the last (``end``) or first bytes of ``theirs``."""
+    t, o = a[theirs], a[ours]
+    span = (t.shape[0] - 1) * t.stride(0) * t.element_size() + t[0].numel() * t.element_size()
+    own = o.numel() * o.element_size()
+    pool = fake(span + own + 64, dtype=torch.uint8)
+    at = (span - 1) // 16 * 16 if end else 0
+    if t.is_contiguous():
+        theirs_now = pool[:span].view(t.dtype).view(t.shape)
+    else:
+        theirs_now = pool[:(t.shape[0] - 1) * t.stride(0) * t.element_size() + t.stride(0) * t.element_size()].view(t.dtype) \
+            .view(t.shape[0], -1)[:, :t.shape[1]]
+    return dict(a, **{theirs: theirs_now, ours: pool[at:at + own].view(o.dtype).view(o.shape)})
+
+
+@pytest.mark.parametrize("end", [False, True])
+@pytest.mark.parametrize("ours,theirs", [("k_tiles", "k"), ("k_tiles", "v"), ("v_tiles", "k"), ("v_tiles", "v"), ("k_tiles", "slots"),
+                                         ("v_tiles", "slots"), ("k_tiles", "v_tiles"), ("k_tiles", "status"), ("status", "slots")])
+def test_rows_into_what_the_call_reads_are_refused(real_ops, ours, theirs, end):
+    with pytest.raises(real_ops.KernelArgumentError, match="overlaps"):
+        real_ops.kv_append_4bit(**_over(_append_args(), ours, theirs, end))
+
+
+@pytest.mark.parametrize("end", [False, True])
+@pytest.mark.parametrize("ours,theirs", [("k_out", "k_tiles"), ("k_out", "v_tiles"), ("v_out", "k_tiles"), ("v_out", "v_tiles"),
+                                         ("k_out", "slots"), ("v_out", "slots"), ("k_out", "status"), ("status", "v_tiles")])
+def test_rows_back_over_what_the_call_reads_are_refused(real_ops, ours, theirs, end):
+    a = _append_args()
+    a["k_out"], a["v_out"] = a.pop("k"), a.pop("v")
+    with pytest.raises(real_ops.KernelArgumentError, match="overlaps"):
+        real_ops.kv_read_4bit(**_over(a, ours, theirs, end))
