@@ -51,7 +51,15 @@ PRB_API int prb_attention_4bit(void* out, long out_stride, const void* q, long q
     if ((uintptr_t)k_tiles % 16 != 0 || (uintptr_t)v_tiles % 16 != 0) return PRB_E_ALIGN;
     if (dtype != PRB_F32 && dtype != PRB_BF16) return PRB_E_DTYPE;
     const int size = dtype == PRB_F32 ? 4 : 2, hpg = heads / kv_heads;
-    if (!prb_rows_apart(out, out_stride * size, q, q_stride * size, n_tokens, (long)heads * head_dim * size))
+    const long width = (long)heads * head_dim * size, word = sizeof(int);
+    const long pool = num_pages * (long)kv_heads * cache4::tile_bytes(head_dim, page_size);
+    const PrbRange rows_out{out, prb_span(n_tokens, out_stride * size, width)}, said{status, 4 * word};
+    const PrbRange queries{q, prb_span(n_tokens, q_stride * size, width)}, keys{k_tiles, pool}, values{v_tiles, pool};
+    const PrbRange table{block_table, (long)n_requests * max_pages * word}, places{positions, n_tokens * word};
+    const PrbRange reqs{tile_req, n_tiles * word}, firsts{tile_row0, n_tiles * word}, counts{tile_rows, n_tiles * word};
+    if (!prb_rows_apart(out, out_stride * size, q, q_stride * size, n_tokens, width) ||
+        !prb_apart({rows_out, said}, {keys, values, table, places, reqs, firsts, counts, {tile_count, word}}) ||
+        prb_overlap(said, queries))
         return PRB_E_OVERLAP;
     attn4::Args p{};
     p.out = out; p.out_stride = out_stride; p.q = q; p.q_stride = q_stride;

@@ -2826,13 +2826,14 @@ def attention_4bit(out, q, k_tiles, v_tiles, block_table, positions, tile_req, t
     (:func:`kv_append_4bit`), the tokens' own keys and values included.
 
     ``q``, ``out``: [T, n_heads * head_dim], both bfloat16 or both float32, of memory of their own (may be column
-    slices of one tensor); ``block_table``
-    int32 [requests, pages a request]; ``positions`` int32 [T].  Tile i: tokens ``tile_row0[i]`` to ``tile_row0[i] +
-    tile_rows[i] - 1``, neighbours of request ``tile_req[i]`` (a row of the block table) at neighbouring positions;
-    no tile has more than ``tile_most`` of them, and 128 rows (tokens times the heads that share a key/value head) a
-    tile are about what a portion of a prompt should be cut into; a decoded token is a tile of one.  ``tile_count``:
-    int32 on the device, how many of the tiles count (all by default).  ``scale`` (of q . k): above 0, float32 up to 1e37.  ``window``: a
-    token sees its last ``window`` positions only.  ``max_context``: the most positions a request holds (the keys are cut into parts by it).
+    slices of one tensor; ``out`` shares memory with nothing else of the call either); ``block_table`` int32 [requests,
+    pages a request]; ``positions`` int32 [T].  Tile i: tokens ``tile_row0[i]`` to ``tile_row0[i] + tile_rows[i] - 1``,
+    neighbours of request ``tile_req[i]`` (a row of the block table) at neighbouring positions; no tile has more than
+    ``tile_most`` of them, and 128 rows (tokens times the heads that share a key/value head) a tile are about what a
+    portion of a prompt should be cut into; a decoded token is a tile of one.  ``tile_count``: int32 on the device, how
+    many of the tiles count (all by default).  ``scale`` (of q . k): above 0, float32 up to 1e37.  ``window``: a token
+    sees its last ``window`` positions only.  ``max_context``: the most positions a request holds (the keys are cut into
+    parts by it).
     ``parts``: CTAs that share a tile's keys (0: the kernel's rule).  Rows of no tile stay as they were."""
     what = "attention_4bit"
     device = q.get_device()

@@ -187,7 +187,7 @@ PRB_API int prb_step_tables(const int* rows, const int* held, const int* brought
     const long word = sizeof(int), n = n_requests, table = n_rows * (long)max_pages;
     if (!prb_apart({{q_start, (n + 1) * word}, {kv_len, n * word}, {positions, t_cap * word}, {seq_of_token, t_cap * word},
                     {slots, t_cap * word}, {block_table, n * max_pages * word}, {tables, table * word},
-                    {n_free >= 0 ? free_next : nullptr, word}},
+                    {n_free >= 0 ? free_next : nullptr, word}, {status, 4 * word}},
                    {{rows, n * word}, {held, n * word}, {brought, n * word}, {free_pages, n_free * word},
                     {n_free >= 0 ? free_start : nullptr, word}}))
         return PRB_E_OVERLAP;

@@ -521,7 +521,7 @@ PRB_API int prb_verify_drafts(int* tokens, int* accepted, const float* logits, l
     if (n_requests <= 0 || n_rows <= 0) return 0;
     if (vocab <= 0 || n_requests > 0x7fffffff / PARTS) return PRB_E_SIZE;
     const long word = 4, width = vocab * word;
-    if (!prb_apart({{tokens, n_rows * word}, {accepted, n_requests * word}},
+    if (!prb_apart({{tokens, n_rows * word}, {accepted, n_requests * word}, {status, 4 * word}},
                    {{row_start, (n_requests + 1) * word}, {drafted, n_rows * word}, {uniforms, 2 * n_rows * word},
                     {temperature, n_requests * word}, {logits, prb_span(n_rows, logits_stride * word, width)},
                     {draft_probs, prb_span(n_rows, probs_stride * word, width)}}))

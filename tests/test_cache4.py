@@ -333,3 +333,24 @@ def test_rows_back_over_what_the_call_reads_are_refused(real_ops, ours, theirs, 
     a["k_out"], a["v_out"] = a.pop("k"), a.pop("v")
     with pytest.raises(real_ops.KernelArgumentError, match="overlaps"):
         real_ops.kv_read_4bit(**_over(a, ours, theirs, end))
+
+
+@pytest.mark.parametrize("end", [False, True])
+@pytest.mark.parametrize("ours,theirs", [("out", n) for n in ("k_tiles", "v_tiles", "block_table", "positions", "tile_req",
+                                                              "tile_row0", "tile_rows", "tile_count", "status")] +
+                         [("status", "q"), ("status", "k_tiles"), ("status", "block_table")])
+def test_attention_over_what_the_call_reads_is_refused(real_ops, ours, theirs, end):
+    with pytest.raises(real_ops.KernelArgumentError, match="overlaps"):
+        real_ops.attention_4bit(**_over(_attention_args(tile_count=fake(1)), ours, theirs, end))
+
+
+@pytest.mark.parametrize("name", ["rows", "held", "brought", "tables", "slots", "block_table", "free_pages"])
+def test_a_status_word_within_a_steps_tables_is_refused(real_ops, name):
+    with pytest.raises(real_ops.KernelArgumentError, match="overlaps"):
+        real_ops.step_tables(**_over(_table_args(), "status", name, False))
+
+
+@pytest.mark.parametrize("name", ["tokens", "accepted", "logits", "drafted", "uniforms", "temperature", "row_start"])
+def test_a_status_word_within_what_is_verified_is_refused(real_ops, name):
+    with pytest.raises(real_ops.KernelArgumentError, match="overlaps"):
+        real_ops.verify_drafts(**_over(_verify_args(), "status", name, False))
