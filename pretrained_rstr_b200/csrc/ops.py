@@ -247,7 +247,7 @@ def _declare(h: ctypes.CDLL) -> None:
     h.prb_kv_append_4bit.argtypes = [P, P, P, L, P, L, P, I, I, I, I, I, I, P, P]
     h.prb_kv_read_4bit.argtypes = [P, L, P, L, P, P, P, I, I, I, I, I, I, P, P]
     h.prb_attention_4bit.argtypes = [P, L, P, L] + [P] * 8 + [I] * 10 + [F, I, I, I, I, P, P]
-    h.prb_step_tables.argtypes = [P] * 13 + [I] * 6 + [P, P]
+    h.prb_step_tables.argtypes = [P] * 15 + [I] * 6 + [P, P]
     h.prb_verify_drafts.argtypes = [P, P, P, L, P, P, P, L, P, P, I, I, I, P, P]
     for name in ("prb_kv_append_4bit", "prb_kv_read_4bit", "prb_attention_4bit", "prb_step_tables",
                  "prb_verify_drafts"):
@@ -2878,7 +2878,7 @@ def attention_4bit(out, q, k_tiles, v_tiles, block_table, positions, tile_req, t
 
 
 def step_tables(rows, held, brought, tables, page_size: int, q_start, kv_len, positions, seq_of_token, slots, block_table,
-                status, free_pages=None, free_start=None, free_next=None) -> None:
+                status, free_pages=None, free_start=None, free_next=None, have_pages=None, have_next=None) -> None:
     """The arrays of a step (as ``engine.batch`` lays them out) from the requests' lengths, on the device.
 
     Request b (row ``rows[b]`` of ``tables`` int32 [rows, pages a request]; no two requests have one row) holds
@@ -2887,12 +2887,15 @@ def step_tables(rows, held, brought, tables, page_size: int, q_start, kv_len, po
     ``block_table`` [requests, pages a request]: the request's pages up to its last new token, -1 behind them.  Pages a
     request grows into come from ``free_pages`` [``free_start[0]`` ...], in the requests' order, and are put into
     ``tables`` too; ``free_next[0]`` becomes the place behind the last one taken (not ``free_start`` itself: the caller
-    has the two take turns).  What a row holds behind its request's ``held`` tokens is overwritten, not used: where
-    requests give tokens back (refused drafts), their pages are better reserved beforehand.  Without ``free_pages`` the
-    rows of ``tables`` hold the pages already (the cache manager reserves them on the host).  No tensor that is written
-    shares memory with another one (the new lengths cannot take the place of ``held``).
+    has the two take turns, or copies one to the other behind the call, in a captured graph too).  What a row holds behind
+    the pages of its request's ``held`` tokens is overwritten, not used, unless ``have_pages`` [requests] says how many
+    pages of its row a request has: where requests give tokens back (refused drafts), the pages that they took for them
+    are theirs still and are used before the list is.  ``have_next`` [requests] becomes the count behind the step, and
+    the two take turns as well.  Without ``free_pages`` the rows of ``tables`` hold the pages already (the cache manager
+    reserves them on the host).  No tensor that is written shares memory with another one (the new lengths cannot take
+    the place of ``held``).
 
-    In the status word: a request whose row or lengths do not fit (it brings nothing, its block table row stays
+    In the status word: a request whose row, lengths or pages do not fit (it brings nothing, its block table row stays
     empty), a page that is missing (the slot is -1), more tokens than token rows (those behind are left out)."""
     what = "step_tables"
     device = held.get_device()
@@ -2902,10 +2905,13 @@ def step_tables(rows, held, brought, tables, page_size: int, q_start, kv_len, po
             block_table.get_device() != device or (status is not None and status.get_device() != device) or \
             (free_pages is not None and free_pages.get_device() != device) or \
             (free_start is not None and free_start.get_device() != device) or \
-            (free_next is not None and free_next.get_device() != device):
+            (free_next is not None and free_next.get_device() != device) or \
+            (have_pages is not None and have_pages.get_device() != device) or \
+            (have_next is not None and have_next.get_device() != device):
         _elsewhere(what, "held rows brought tables q_start kv_len positions seq_of_token slots block_table status "
-                   "free_pages free_start free_next", held, rows, brought, tables, q_start, kv_len, positions, seq_of_token,
-                   slots, block_table, status, free_pages, free_start, free_next)
+                   "free_pages free_start free_next have_pages have_next", held, rows, brought, tables, q_start, kv_len,
+                   positions, seq_of_token, slots, block_table, status, free_pages, free_start, free_next, have_pages,
+                   have_next)
     n, cap = held.numel(), positions.numel()
     if not 1 <= n <= STEP_TABLES_MAX_REQUESTS:
         raise KernelArgumentError(f"{what}: takes 1 to {STEP_TABLES_MAX_REQUESTS} requests, got {n}")
@@ -2927,10 +2933,15 @@ def step_tables(rows, held, brought, tables, page_size: int, q_start, kv_len, po
         start_at, next_at = _ints(what, "free_start", free_start, 1), _ints(what, "free_next", free_next, 1)
         if start_at == next_at:
             raise KernelArgumentError(f"{what}: free_next must not be free_start")
+    have_at = have_next_at = None
+    if have_pages is not None or have_next is not None:
+        if have_pages is None or have_next is None or free_pages is None:
+            raise KernelArgumentError(f"{what}: have_pages and have_next come together, with free_pages")
+        have_at, have_next_at = _ints(what, "have_pages", have_pages, n), _ints(what, "have_next", have_next, n)
     _launch_on(device, what, "prb_step_tables",
                _ints(what, "rows", rows, n), _ints(what, "held", held, n), _ints(what, "brought", brought, n), t_at,
-               free_at, start_at, next_at, _ints(what, "q_start", q_start, n + 1), _ints(what, "kv_len", kv_len, n),
-               _ints(what, "positions", positions, 0), _ints(what, "seq_of_token", seq_of_token, cap),
+               free_at, start_at, next_at, have_at, have_next_at, _ints(what, "q_start", q_start, n + 1),
+               _ints(what, "kv_len", kv_len, n), _ints(what, "positions", positions, 0), _ints(what, "seq_of_token", seq_of_token, cap),
                _ints(what, "slots", slots, cap), b_at, n, lanes, cap, wide, page_size, n_free,
                None if status is None else _ints(what, "status", status, 4))
 

@@ -6,7 +6,8 @@
 //   q_start[b]  = tokens of the requests before b         kv_len[b] = held[b] + brought[b]
 //   pages of b  : ceil(held / page) it has, ceil(kv_len / page) it needs; what it lacks comes from
 //                 free_pages[free_start + (pages taken by the requests before b)], and on
-//                 (without a list its row holds them already)
+//                 (without a list its row holds them already; with have_pages it has as many as that says, where that is
+//                 more: those it took for tokens that did not stay)
 //   token t of b: position held[b] + (t - q_start[b]), slot page(position / page) * page + position % page
 //
 // Bound by its launch for a decode step (64 requests of up to 16 pages: 3.3 us) and by the look-ups of the sums and the
@@ -30,6 +31,8 @@ struct TableArgs {
     const int* free_pages;
     const int* free_start;
     int* free_next;
+    const int* have_pages;                   // null: none behind those that the held tokens lie in
+    int* have_next;
     int* q_start;
     int* kv_len;
     int* positions;
@@ -47,7 +50,7 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const TableArgs p)
     extern __shared__ int shared[];
     int* tok = shared;                       // [n + 1] tokens before each request
     int* fresh = tok + p.n_requests + 1;     // [n + 1] new pages before each request
-    int* have = fresh + p.n_requests + 1;    // [n] pages that its row holds already, or -1: the request is refused
+    int* have = fresh + p.n_requests + 1;    // [n] pages of its row that the step reads from it, or -1: the request is refused
     __shared__ int sums[2][THREADS / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const bool speaks = blockIdx.x == 0;     // one CTA reports and writes what there is one of
@@ -60,14 +63,15 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const TableArgs p)
     int t_sum = 0, f_sum = 0;
     for (int b = b0; b < b1; ++b) {
         const int row = p.rows[b], held = p.held[b], brought = p.brought[b];
-        const bool fine = row >= 0 && row < p.n_rows && held >= 0 && brought >= 0 &&
+        const int own = p.have_pages != nullptr ? p.have_pages[b] : 0;
+        const bool fine = row >= 0 && row < p.n_rows && held >= 0 && brought >= 0 && own >= 0 && own <= p.max_pages &&
                           (long)held + brought <= (long)p.max_pages * p.page_size;
         if (!fine && speaks) {
             if (row < 0 || row >= p.n_rows) prb_set_status(p.status, PRB_S_ROW_RANGE, b, row, p.n_rows);
             else prb_set_status(p.status, PRB_S_POSITION_RANGE, b, held, brought);
         }
         const int w = fine ? (int)(((long)held + brought + p.page_size - 1) / p.page_size) : -1;
-        const int h = !fine ? -1 : p.n_free >= 0 ? (int)(((long)held + p.page_size - 1) / p.page_size) : w;
+        const int h = !fine ? -1 : p.n_free >= 0 ? min(max((int)(((long)held + p.page_size - 1) / p.page_size), own), w) : w;
         have[b] = h;
         tok[b] = t_sum;                      // (within the thread's run, for now)
         fresh[b] = f_sum;
@@ -122,13 +126,19 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const TableArgs p)
         for (int b = threadIdx.x; b < p.n_requests; b += THREADS) {
             p.q_start[b] = min(tok[b], p.t_cap);
             p.kv_len[b] = have[b] < 0 ? 0 : p.held[b] + p.brought[b];
+            if (p.have_next != nullptr) {
+                // pages that it has and those it takes, as far as the list goes; a refused one has what it had
+                const long left = start < 0 ? 0 : (long)p.n_free - start - fresh[b];
+                const int taken = (int)min(max(left, 0L), (long)(fresh[b + 1] - fresh[b]));
+                p.have_next[b] = have[b] < 0 ? p.have_pages[b] : max(p.have_pages[b], have[b] + taken);
+            }
         }
         if (threadIdx.x == 0) {
             p.q_start[p.n_requests] = min(t_total, p.t_cap);
             if (t_total > p.t_cap) prb_set_status(p.status, PRB_S_ROW_RANGE, -1, t_total, p.t_cap);
-            if (p.n_free >= 0) *p.free_next = add(max(start, 0), f_total);
+            if (p.n_free >= 0) *p.free_next = add(min(max(start, 0), MOST), f_total);
             if (f_total > 0 && (start < 0 || (long)start + f_total > p.n_free))
-                prb_set_status(p.status, PRB_S_PAGE_RANGE, -1, start + f_total, p.n_free);
+                prb_set_status(p.status, PRB_S_PAGE_RANGE, -1, add(min(max(start, -1), MOST), f_total), p.n_free);
         }
     }
 
@@ -175,24 +185,26 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const TableArgs p)
 }  // namespace
 
 PRB_API int prb_step_tables(const int* rows, const int* held, const int* brought, int* tables, const int* free_pages,
-                            const int* free_start, int* free_next, int* q_start, int* kv_len, int* positions,
-                            int* seq_of_token, int* slots, int* block_table, int n_requests, int n_rows, int t_cap,
+                            const int* free_start, int* free_next, const int* have_pages, int* have_next, int* q_start,
+                            int* kv_len, int* positions, int* seq_of_token, int* slots, int* block_table, int n_requests,
+                            int n_rows, int t_cap,
                             int max_pages, int page_size, int n_free, int* status, cudaStream_t stream) {
     if (n_requests <= 0 || n_requests > MAX_REQUESTS || n_rows <= 0 || t_cap < 0 || t_cap > MOST || max_pages <= 0 ||
         page_size <= 0 || (long)max_pages * page_size > 0x7fffffffL)
         return PRB_E_SIZE;
     if (n_free >= 0 && (free_start == nullptr || free_next == nullptr || (n_free > 0 && free_pages == nullptr)))
         return PRB_E_ARG;
+    if ((have_pages == nullptr) != (have_next == nullptr) || (have_pages != nullptr && n_free < 0)) return PRB_E_ARG;
     // (a CTA may still read what another writes: the new lengths, for one, must not take the place of those held)
     const long word = sizeof(int), n = n_requests, table = n_rows * (long)max_pages;
     if (!prb_apart({{q_start, (n + 1) * word}, {kv_len, n * word}, {positions, t_cap * word}, {seq_of_token, t_cap * word},
                     {slots, t_cap * word}, {block_table, n * max_pages * word}, {tables, table * word},
-                    {n_free >= 0 ? free_next : nullptr, word}, {status, 4 * word}},
+                    {n_free >= 0 ? free_next : nullptr, word}, {have_next, n * word}, {status, 4 * word}},
                    {{rows, n * word}, {held, n * word}, {brought, n * word}, {free_pages, n_free * word},
-                    {n_free >= 0 ? free_start : nullptr, word}}))
+                    {n_free >= 0 ? free_start : nullptr, word}, {have_pages, n * word}}))
         return PRB_E_OVERLAP;
-    const TableArgs a{rows, held, brought, tables, free_pages, free_start, free_next, q_start, kv_len, positions,
-                      seq_of_token, slots, block_table, n_requests, n_rows, t_cap, max_pages, page_size, n_free, status};
+    const TableArgs a{rows, held, brought, tables, free_pages, free_start, free_next, have_pages, have_next, q_start,
+                      kv_len, positions, seq_of_token, slots, block_table, n_requests, n_rows, t_cap, max_pages, page_size, n_free, status};
     const int shared = (3 * n_requests + 2) * (int)sizeof(int);
     const cudaError_t a_err = prb_allow_shared<step_tables_kernel>((3 * MAX_REQUESTS + 2) * (int)sizeof(int));
     if (a_err != cudaSuccess) return (int)a_err;

@@ -354,3 +354,21 @@ def test_a_status_word_within_a_steps_tables_is_refused(real_ops, name):
 def test_a_status_word_within_what_is_verified_is_refused(real_ops, name):
     with pytest.raises(real_ops.KernelArgumentError, match="overlaps"):
         real_ops.verify_drafts(**_over(_verify_args(), "status", name, False))
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(have_pages=fake(3)), "come together"), (dict(have_next=fake(3)), "come together"),
+    (dict(have_pages=fake(3), have_next=fake(3), free_pages=None, free_start=None, free_next=None), "with free_pages"),
+    (dict(have_pages=fake(2), have_next=fake(3)), "have_pages"), (dict(have_pages=fake(3), have_next=fake(2)), "have_next"),
+    (dict(have_pages=fake(3, dtype=torch.int64), have_next=fake(3)), "have_pages"),
+    (dict(have_pages=fake(3), have_next=torch.zeros(3, dtype=torch.int32)), "have_next is not on")])
+def test_counts_of_pages_refused(ops, change, word):
+    with pytest.raises(ops.KernelArgumentError, match=word):
+        ops.step_tables(**_table_args(**change))
+
+
+@pytest.mark.parametrize("theirs", ["have_pages", "held", "rows", "kv_len", "tables", "free_pages"])
+def test_counts_of_pages_that_share_memory_are_refused(real_ops, theirs):
+    a = _table_args(have_pages=fake(3), have_next=fake(3))
+    with pytest.raises(real_ops.KernelArgumentError, match="overlaps"):
+        real_ops.step_tables(**_over(a, "have_next", theirs, False))

@@ -218,3 +218,92 @@ def test_values_next_to_the_largest_number(d, page, parts):
     ref, b = ref.view(new, kv, d), b.view(new, kv, d)
     # the value (3.409e38 in the cache, 3.390e38 the largest number), half a step of the result (2^-8)
     assert bool(((got.double() - ref).abs()[seen] <= ((0.0057 + 1.01 * 2.0 ** -8) * b)[seen]).all())
+
+
+# ------------------------------------------------------------------------------------ tables
+@pytest.mark.parametrize("captured", [False, True])
+def test_pages_taken_for_refused_tokens_are_used_by_the_next_step(captured):
+    """Steps that bring drafted tokens and keep some, with pages from a list: a page a request took stays its own, the list
+    gives no more than the requests ever held, no page is given twice, and nothing comes to the host."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(1)
+    n, page, wide, lanes, rounds, drafts = 70, 16, 12, 75, 40, 7
+    lane = torch.randperm(lanes, generator=g)[:n].tolist()
+    free = torch.randperm(n * wide + 9, generator=g).tolist()
+    kept = torch.randint(0, drafts + 2, (rounds, n), generator=g)          # of the drafted tokens and the one before them
+    kept[:, 0] = 0                                                        # (a request that refuses everything)
+    cap = n * (drafts + 1)
+    tables, held, brought = _ints([[-1] * wide] * lanes), _ints([0] * n), _ints([drafts + 1] * n)
+    have, have_next, start, nxt = _ints([0] * n), _ints([-1] * n), _ints([4]), _ints([-1])
+    out = dict(q_start=_ints([0] * (n + 1)), kv_len=_ints([0] * n), positions=_ints([0] * cap), seq_of_token=_ints([0] * cap),
+               slots=_ints([0] * cap), block_table=_ints([[0] * wide] * n))
+    status, step_kept, lane_d, free_d = _status(), _ints([0] * n), _ints(lane), _ints(free)
+
+    def one_round():
+        ops.step_tables(lane_d, held, brought, tables, page, *out.values(), status, free_pages=free_d, free_start=start,
+                        free_next=nxt, have_pages=have, have_next=have_next)
+        start.copy_(nxt)
+        have.copy_(have_next)
+        held.add_(step_kept)
+    go = one_round
+    if captured:
+        first = [t.clone() for t in (tables, held, have, start)]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            one_round()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            one_round()
+        for t, was in zip((tables, held, have, start), first):
+            t.copy_(was)
+        go = graph.replay
+    length, pages, at = [0] * n, [[] for _ in range(n)], 4
+    for r in range(rounds):
+        fits = [min(drafts + 1, wide * page - x) for x in length]
+        brought.copy_(torch.tensor(fits, dtype=torch.int32))
+        step_kept.copy_(torch.minimum(kept[r].to(torch.int32), torch.tensor(fits, dtype=torch.int32)))
+        go()
+        want_slots = []
+        for b in range(n):
+            need = -(-(length[b] + fits[b]) // page)
+            while len(pages[b]) < need:
+                pages[b].append(free[at])
+                at += 1
+            want_slots += [pages[b][x // page] * page + x % page for x in range(length[b], length[b] + fits[b])]
+        assert status.tolist() == [0] * 4
+        assert out["slots"].tolist() == want_slots + [-1] * (cap - len(want_slots))
+        needs = [-(-(x + f) // page) for x, f in zip(length, fits)]
+        assert out["block_table"].tolist() == [(p[:m] + [-1] * wide)[:wide] for p, m in zip(pages, needs)]
+        assert have.tolist() == [len(p) for p in pages] and start.tolist() == [at]
+        length = [x + min(int(k), f) for x, k, f in zip(length, kept[r], fits)]
+        assert held.tolist() == length
+    flat = [p for own in pages for p in own]
+    assert len(flat) == len(set(flat)) == at - 4
+    table = tables.tolist()
+    assert all(table[row][:len(p)] == p for row, p in zip(lane, pages))
+
+
+def test_pages_a_row_cannot_hold_are_reported():
+    ops = _ops()
+
+    def go(held, have, start=0):
+        n = len(held)
+        table, status, nxt, have_next = _ints([[5, 6, -1]] * n), _status(), _ints([-1]), _ints([-9] * n)
+        o = [_ints([9] * k) for k in (n + 1, n, 8, 8, 8)]
+        ops.step_tables(_ints(list(range(n))), _ints(held), _ints([2] * n), table, 16, *o, _ints([[9] * 3] * n), status,
+                        free_pages=_ints([20, 21, 22]), free_start=_ints([start]), free_next=nxt, have_pages=_ints(have),
+                        have_next=have_next)
+        return [x.tolist() for x in o], table.tolist(), nxt.tolist(), have_next.tolist(), status.tolist()
+    o, table, nxt, have_next, status = go([30, 3], [4, 1])                # more pages than a row has places
+    assert status[:3] == [2, 0, 30] and o[0] == [0, 0, 2] and o[1] == [0, 5] and have_next == [4, 1] and nxt == [0]
+    o, table, nxt, have_next, status = go([30, 3], [-1, 1])
+    assert status[0] == 2 and o[1] == [0, 5] and have_next == [-1, 1]
+    # fewer than its tokens lie in: those it has are looked up as without the count
+    o, table, nxt, have_next, status = go([31, 3], [0, 1])
+    assert status == [0] * 4 and table == [[5, 6, 20], [5, 6, -1]] and have_next == [3, 1] and nxt == [1]
+    assert o[4][:2] == [6 * 16 + 15, 20 * 16]
+    # a list that has run out: what is missing is not counted
+    o, table, nxt, have_next, status = go([31, 3], [2, 1], start=3)
+    assert status[0] == 4 and have_next == [2, 1] and o[4][:2] == [6 * 16 + 15, -1]
