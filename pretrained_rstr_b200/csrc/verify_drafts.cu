@@ -518,8 +518,8 @@ PRB_API int prb_verify_drafts(int* tokens, int* accepted, const float* logits, l
                               const int* drafted, const float* draft_probs, long probs_stride, const float* uniforms,
                               const float* temperature, int n_requests, int n_rows, int vocab, int* status,
                               cudaStream_t stream) {
-    if (n_requests <= 0 || n_rows <= 0) return 0;
-    if (vocab <= 0 || n_requests > 0x7fffffff / PARTS) return PRB_E_SIZE;
+    if (n_requests <= 0) return 0;                            // (requests of no rows are recorded by the kernel)
+    if (n_rows < 0 || vocab <= 0 || n_requests > 0x7fffffff / PARTS) return PRB_E_SIZE;
     const long word = 4, width = vocab * word;
     if (!prb_apart({{tokens, n_rows * word}, {accepted, n_requests * word}, {status, 4 * word}},
                    {{row_start, (n_requests + 1) * word}, {drafted, n_rows * word}, {uniforms, 2 * n_rows * word},

@@ -109,6 +109,16 @@ def test_a_request_of_too_many_rows_has_no_tokens(rows):
     assert tokens == drafted[:2] + [-1] * rows + drafted[-2:]
 
 
+def test_requests_of_no_rows_accept_nothing():
+    """Recorded, with the others as they are; without any row at all too."""
+    logits = torch.randn(3, 50, generator=torch.Generator().manual_seed(0))
+    best = logits.argmax(-1).tolist()
+    (tokens, accepted), status = _verify(logits, [0, 0, 3, 3], best, torch.zeros(3, 2), [0.0] * 3)
+    assert status[0] == 6 and (tokens, accepted) == (best, [0, 2, 0])
+    (tokens, accepted), status = _verify(logits[:0], [0, 0, 0], [], torch.zeros(0, 2), [0.0, 1.0])
+    assert status[0] == 6 and (tokens, accepted) == ([], [0, 0])
+
+
 # ------------------------------------------------------------------------------------ attention
 def _cached(k, v, page):
     n, kv, d = k.shape
@@ -134,6 +144,25 @@ def _attend(k, v, q, held, page, scale, parts=0, window=None, status_word=0):
                        min(new, most), heads, d, page, scale, window, total, status, parts=parts)
     assert status.tolist()[0] == status_word
     return out.float().cpu().view(new, heads, d)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv,d,page", [(2, 2, 64, 64), (4, 1, 128, 64), (2, 1, 96, 32), (3, 3, 16, 16)])
+@pytest.mark.parametrize("held,new,parts", [(64, 1, 0), (256, 1, 4), (186, 70, 0), (186, 70, 4), (250, 40, 2), (316, 6, 8)])
+def test_a_key_that_is_no_number_alone_in_its_part(held, new, parts, heads, kv, d, page, dtype):
+    """The first token that opens a block of 64 has keys that are no numbers: the part of the keys that holds nothing else
+    for it still makes its result NaN."""
+    g = torch.Generator().manual_seed(held)
+    total = held + new
+    bad = -(-held // 64) * 64
+    k, v, q = torch.randn(total, kv, d, generator=g), torch.randn(total, kv, d, generator=g), torch.randn(new, heads * d, generator=g)
+    want = _attend(k, v, q.to(dtype), held, page, 0.2, parts)
+    k[bad, 0, 3] = math.nan
+    got = _attend(k, v, q.to(dtype), held, page, 0.2, parts)
+    nan = torch.zeros(new, heads, d, dtype=torch.bool)
+    nan[bad - held:, :heads // kv] = True
+    assert torch.equal(torch.isnan(got), nan)
+    assert torch.equal(got[~nan], want[~nan])
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
