@@ -228,8 +228,8 @@ def test_weights_meet_middles_unrounded(heads, kv, d, page, held, new, window):
 
 @pytest.mark.parametrize("d,page,parts", [(64, 64, 1), (64, 64, 4), (128, 64, 1), (48, 32, 1)])
 def test_values_next_to_the_largest_number(d, page, parts):
-    """A float32 number beyond bfloat16's largest one, whose code stands for more than that: who does not see it keeps its result, who
-    sees it gets what the formula says within the roundings."""
+    """A float32 number beyond bfloat16's largest one, whose code stands for more than that: a portion of a prompt has no number
+    for it where it is seen, and what it was where it is not."""
     g = torch.Generator().manual_seed(d)
     held, new, kv = 150, 60, 2
     k, v = (torch.randn(held + new, kv, d, generator=g) for _ in range(2))
@@ -241,12 +241,7 @@ def test_values_next_to_the_largest_number(d, page, parts):
     seen = torch.zeros(new, kv, d, dtype=torch.bool)
     seen[at - held:, 0, :32] = True
     assert torch.equal(got[~seen], want[~seen])
-    kt, vt, table = _cached(k, v, page)
-    ref, (_a, b, _e) = plain.attention(q.cpu(), kt.cpu(), vt.cpu(), table.tolist(), list(range(held, held + new)), [0] * new, kv, d, page,
-                                       0.2, None)
-    ref, b = ref.view(new, kv, d), b.view(new, kv, d)
-    # the value (3.409e38 in the cache, 3.390e38 the largest number), half a step of the result (2^-8)
-    assert bool(((got.double() - ref).abs()[seen] <= ((0.0057 + 1.01 * 2.0 ** -8) * b)[seen]).all())
+    assert not bool(torch.isfinite(got[seen]).any())
 
 
 # ------------------------------------------------------------------------------------ tables
