@@ -19,9 +19,9 @@
 // it; its exponentials (exp64: 20 operations of 64 bits) are taken once and kept in shared memory where they fit.
 // 256 threads, so that four CTAs fit an SM and the clusters of 64 requests run side by side.
 //
-// 64 requests of 5 rows of 50,257: 42 us, of which a CTA spends 13 to 17 on the rows (64 MB are 10 us' worth), 5 on who stays
+// 64 requests of 5 rows of 50,257: 41 us, of which a CTA spends 13 to 17 on the rows (64 MB are 10 us' worth), 5 on who stays
 // and 15 on the drawn row, where it waits for the others three times; without a draw (temperature 0) 22 us.  One request
-// of 5 rows 19 us, of which 10 on the drawn row.
+// of 5 rows 20 us, of which 10 on the drawn row.
 #include "common.cuh"
 #include "ranges.cuh"
 #include "tcgen05.cuh"
@@ -203,16 +203,26 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, AHEAD_R
                 return;
             }
             // The largest first, then the lowest place that has it (places go up within a batch and from batch to batch): one
-            // request of 4 rows of 50,257 takes 9.4 us a call, with `better` number by number 13.0.
-            float most = v[0];
+            // request of 4 rows of 50,257 takes 9.0 us a call, with `better` number by number 13.0.
+            float quads[BATCH];
 #pragma unroll
-            for (int k = 1; k < 4 * BATCH; ++k) most = max_nan(most, v[k]);
+            for (int k = 0; k < BATCH; ++k)
+                quads[k] = max_nan(max_nan(v[4 * k], v[4 * k + 1]), max_nan(v[4 * k + 2], v[4 * k + 3]));
+            float most = quads[0];
+#pragma unroll
+            for (int k = 1; k < BATCH; ++k) most = max_nan(most, quads[k]);
             const bool none = most != most;
             if (i >= vecs || !(none ? top == top : most > top || index == 0x7fffffff)) return;
             int at = 0;
+            if (none) {
 #pragma unroll
-            for (int k = 4 * BATCH - 1; k >= 0; --k)
-                if (none ? v[k] != v[k] : v[k] == most) at = 4 * (k / 4) * THREADS + k % 4;
+                for (int k = 4 * BATCH - 1; k >= 0; --k)
+                    if (v[k] != v[k]) at = 4 * (k / 4) * THREADS + k % 4;
+            } else {
+#pragma unroll
+                for (int k = 4 * BATCH - 1; k >= 0; --k)
+                    if (v[k] == most) at = 4 * (k / 4) * THREADS + k % 4;
+            }
             top = most;
             index = lo + head + 4 * i + at;
         };
@@ -300,7 +310,7 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, AHEAD_R
     float top = -INFINITY;
     int best = 0x7fffffff;
     bool stays = false, unsure = false;
-    const double inverse = 1.0 / (double)t;
+    const double inverse = greedy ? 0.0 : 1.0 / (double)t;
     // What the sum in 32 bits may be off by, of itself.  An exponent is off by 2^-23 of itself (the scale's rounding, the
     // product's), and a term of exponent -x weighs 2^-x, so a whole row of them by less than 32 x 2^-23; the exponential by
     // 2^-22, a sum of n terms one after the other by n 2^-24.  Twice that and more is called next to the border.
@@ -328,7 +338,7 @@ __global__ void __cluster_dims__(PARTS, 1, 1) __launch_bounds__(THREADS, AHEAD_R
             } else if (greedy) {
                 stays = x == best;
             } else {
-                const double mine = exp64(((double)p.logits[(long)(r0 + lane) * p.logits_stride + x] - (double)ref) / (double)t);
+                const double mine = exp64(((double)p.logits[(long)(r0 + lane) * p.logits_stride + x] - (double)ref) * inverse);
                 const double theirs = p.draft_probs ? (double)p.draft_probs[(long)(r0 + lane) * p.probs_stride + x] : 1.0;
                 const double bar = (double)p.uniforms[2 * (r0 + lane)] * theirs * (double)sum;
                 stays = bar < mine;
@@ -530,9 +540,9 @@ PRB_API int prb_verify_drafts(int* tokens, int* accepted, const float* logits, l
                        temperature, n_requests, n_rows, vocab, status};
     const int each = (vocab + PARTS - 1) / PARTS;
     const size_t shared = each <= KEPT ? each * sizeof(double) : 0;
-    // The next row asked for ahead takes 110 registers instead of 62, so it is for launches of two CTAs an SM at most.  us
-    // without and with it, 50,257 logits a row: 1 request of 4 rows, greedy, 8.9 and 8.0; 32 of them 11.8 and 10.1; 32 of 5
-    // rows at temperature 0.8 32.0 and 26.8; but 64 of those, where four CTAs an SM do more, 41.2 and 51.2.
+    // The next row asked for ahead takes some 110 registers instead of 60, so it is for launches of two CTAs an SM at most.
+    // us without and with it, 5 rows of 50,257 logits at temperature 0.8: 32 requests 33.2 and 27.4, one request 19.9 either
+    // way; but 64, where four CTAs an SM do more, 41.3 and 52.0.
     const bool ahead = (long)n_requests * PARTS <= 2L * prb_sm_count();
     cudaError_t e = ahead ? prb_allow_shared<verify_kernel<true>>(KEPT * (int)sizeof(double))
                           : prb_allow_shared<verify_kernel<false>>(KEPT * (int)sizeof(double));
