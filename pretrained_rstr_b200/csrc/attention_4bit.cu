@@ -15,8 +15,8 @@ int prb_attention_4bit_rows(const attn4::Args& p, long rows, int max_context, in
 
 namespace {
 // More rows than this go to the tensor-memory kernel where it takes the call: 33 tokens at 300 of 12 heads of 64 20.8 us by
-// the other one, 13.1 by that; 8 x 33 at 1,000 28.0 and 25.5; 16 x 64 at 500 of 16 heads 48.9 and 25.3; 20 x 12 tokens of
-// 4 heads a key/value head of 128 59.5 and 46.6.
+// the other one, 12.6 by that; 8 x 33 at 1,000 33.7 and 25.3; 16 x 64 at 500 of 16 heads 49.8 and 25.1; 20 x 12 tokens at
+// 1,000 of 4 heads a key/value head of 128 61.4 and 46.4.
 constexpr long TILE_ROWS = 32;
 
 // up to 4 rows a tile, or 8

@@ -18,10 +18,11 @@
 // scores' accumulator has keys along lanes where the probabilities' operand has rows there: the rounded numbers change
 // lanes by shuffles (as_operand).
 //
-// What bounds it: the instructions that turn words of codes into operands and scale them (some 900 a stage of 64 keys of 64
-// channels, issued in about half of the cycles: fixed latencies and the ALU take the rest); then the bytes of the cache.
-// 64 tokens at contexts of 500 to 1,000 of 25 heads of 64 (96 MB) take 42.6 us, 2.2 TB/s; 8 at 16,000 to 32,749 of 8 x 128
-// with four rows a key/value head (240 MB) 75 us, 3.2 TB/s; one at 1,000 of 12 heads 6.9 us, a chain of look-ups, two
+// What bounds it: the instructions that turn words of codes into operands and scale them (some 880 a stage of 64 keys of 64
+// channels, issued in about half of the cycles: too few warps to cover their latencies, and units of unequal length in
+// little more than one round of CTAs); then the bytes of the cache.
+// 64 tokens at contexts of 500 to 1,000 of 25 heads of 64 (96 MB) take 41.2 us, 2.3 TB/s; 8 at 16,000 to 32,749 of 8 x 128
+// with four rows a key/value head (240 MB) 74.6 us, 3.2 TB/s; one at 1,000 of 12 heads 6.8 us, a chain of look-ups, two
 // stages and the parts' meeting.
 // With bfloat16 queries the 8 stays in the codes of the keys (128 + c is what the bits of a code make without an
 // addition) and goes with the middle: q . (128 + c) is off by 2^-24 of 136 sums of |q|, which is nothing there.
@@ -45,8 +46,8 @@ constexpr int STAGES = 2;                  // ring buffers of a warp
 constexpr int MAX_PARTS = 8;               // CTAs of a cluster (portable)
 
 // Keys of a stage: 64, or 32 where a thread's scores and results would not fit the registers.  Longer stages and more
-// registers measured better than more warps: 8 x 32,749 positions of 8 x 128 87.5 us with stages of 32 keys and four CTAs an
-// SM, 78.6 with 64 and two; 64 tokens at 1,000 of 25 heads of 64 42 with 64, 51 with 32.
+// registers measured better than more warps: 8 x 32,749 positions of 8 x 128 88.9 us with stages of 32 keys and four CTAs an
+// SM, 74.7 with 64 and two; 64 tokens at 1,000 of 25 heads of 64 41 with 64, 50 with 32.
 __host__ __device__ constexpr int stage_keys(int ng, int qn, bool wide) {
     return (ng <= 2 && qn <= 2) || (qn == 1 && !wide) ? 64 : 32;
 }
@@ -777,9 +778,9 @@ template <int NG, int QN, int EN, typename T> int launch_by(Args p, long rows, i
     if (units > 0x7fffffffL / MAX_PARTS) return PRB_E_SIZE;
     p.subs = (int)subs;
     // Four warps a CTA; two once the units alone fill the SMs with such CTAs: a warp then has twice the stages to
-    // one set-up and half as many states to merge.  64 tokens at 1,000 of 12 heads (768 units) 27.9 us with four, 23.3 with
-    // two; at 300 of 16 heads (1,024) 15.6 and 13.6; 24 x 5 tokens of 16 heads (384) 14.4 and 19.7; float32 texts (more
-    // instructions a stage) 30.9 and 39.8.
+    // one set-up and half as many states to merge.  64 tokens at 1,000 of 12 heads (768 units) 26.7 us with four, 22.2 with
+    // two; at 300 of 16 heads (1,024) 15.2 and 13.0; 24 x 5 tokens of 16 heads (384) 13.9 and 19.2; float32 texts (more
+    // instructions a stage) 32.4 and 41.8.
     const long slots = (long)ctas_of(NG, QN, sizeof(T) == 4) * prb_sm_count();
     p.warps = QN == 1 && sizeof(T) == 2 && units > slots ? 2 : MAX_WARPS;
     // Parts of a unit's keys while all CTAs still run side by side, each with a stage a warp at least.  (The longest

@@ -8,14 +8,16 @@
 //   1      allocates tensor memory; one thread issues tcgen05.mma: S = Q K^T (128 x 64), O += P V;
 //   2-9    softmax: two threads a row, each 32 of a block's 64 scores and half of the output's channels;
 //   10-17  turn codes into operands in the swizzled layout, once for all 128 rows.
-// Values become bfloat16 (2^-8 of a value, as a bfloat16 cache would hold it, on top of the cache's own rounding).  Keys
+// Weights become bfloat16 (2^-8, as before any such product; their sum is of the unrounded ones), and so do values (2^-8 of
+// a value, as a bfloat16 cache would hold it, on top of the cache's own rounding).  Keys
 // become the sum of two bfloat16 numbers and take two products: a key's rounding moves a score by the product of the
 // query's and the key's lengths times it, which at ordinary scores is several times what P's rounding costs, and the tensor
 // cores wait for the softmax anyway.
 //
-// Measured: portions of 4 x 512 tokens at contexts of 4,000, 16 heads of 64 (16.5 GFLOP) 102 us, where tiles of 32 rows on
-// mma.sync take 207; 512 tokens at 8,000 of 32 heads over 8 x 128 (65 GFLOP) 190 us, 340 TFLOP/s.  What bounds it: the
-// instructions of softmax and conversion (6,500 a block of 64 keys, a third of them the conversion, in 70 % of the issue
+// Measured: portions of 4 x 512 tokens at contexts of 4,000, 16 heads of 64 (16.5 GFLOP) 99.5 us, where tiles of 32 rows on
+// mma.sync take 200 (and with a window of 1,000, which only they know, 115); 512 tokens at 8,000 of 32 heads over 8 x 128
+// (65 GFLOP) 185 us, 350 TFLOP/s.  What bounds it: the
+// instructions of softmax and conversion (5,900 a block of 64 keys, a third of them the conversion, in 70 % of the issue
 // slots while a CTA pair runs), and the SMs that one tile less leaves with one CTA where others have two.  Eight warps
 // convert: with four the blocks waited for them (512 tokens at 8,000: 302 us).
 //
@@ -24,8 +26,8 @@
 // and the rows that see it are made NaN in the channels of its group at the end, since a product would spread it over all
 // rows.
 //
-// Every wait is bounded: where one gives up the status word says so, nothing more is stored, copies in flight are waited
-// for, tensor memory is freed.
+// Every wait is bounded: where one gives up the status word says so, its CTA stores nothing more, copies in flight are
+// waited for, tensor memory is freed.
 #include <type_traits>
 
 #include "cache4.cuh"
@@ -689,8 +691,9 @@ int prb_attention_4bit_tile(void* out, long out_stride, const void* q, long q_st
              page_size % 64 == 0 ? 64 : page_size % 32 == 0 ? 32 : 16, scale, 0x43004300u, status};
     const int blocks = (max_context + KB - 1) / KB;
     // Parts of a tile's keys while all CTAs still run side by side (two an SM at head size 64, one at 128), each of at least
-    // eight blocks: 128 tokens at 1,000 of 12 heads (12 units) 27.7 us in one part, 20.1 in two, 15.7 in four; 2 x 1,024
-    // tokens of 12 heads (192 units) 36.5, 37.5 and 48.1; 512 tokens at 8,000 of 8 x 128 (128 units) 185, 200 and 225.
+    // eight blocks: 128 tokens at 1,000 of 12 heads (12 units) 27.4 us in one part, 20.3 in two, 16.0 in four; 2 x 1,024
+    // tokens of 12 heads (192 units) 36.1, 37.9 and 48.5; 512 tokens at 8,000 of 8 x 128 (128 units) 184, 196 and 219.
+    // (Asked for by the call: 1, 2 or 4, whichever is not above it.)
     const long slots = (head_dim <= 64 ? 2L : 1L) * prb_sm_count();
     while (p.parts < MAX_PARTS && units * p.parts * 2 <= slots && blocks >= p.parts * 8) p.parts *= 2;
     if (parts > 0) p.parts = parts >= 4 ? 4 : parts >= 2 ? 2 : 1;

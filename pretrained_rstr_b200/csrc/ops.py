@@ -2834,7 +2834,13 @@ def attention_4bit(out, q, k_tiles, v_tiles, block_table, positions, tile_req, t
     many of the tiles count (all by default).  ``scale`` (of q . k): above 0, float32 up to 1e37.  ``window``: a token
     sees its last ``window`` positions only.  ``max_context``: the most positions a request holds (the keys are cut into
     parts by it).
-    ``parts``: CTAs that share a tile's keys (0: the kernel's rule).  Rows of no tile stay as they were."""
+    ``parts``: CTAs that share a tile's keys (0: the kernel's rule); where bfloat16 tiles may have more than 32 rows and
+    there is no window, 1, 2 or 4 of them, whichever is not above it.  Rows of no tile stay as they were.
+
+    Rounding: bfloat16 results, and of bfloat16 queries each weight times its group's step (2^-8 of that); where tiles may
+    have more than 32 rows and there is no window, each weight and each value (2^-8 of their product, twice), and a value
+    past bfloat16's largest number (3.39e38) makes the results that see it none.  float32: some 1e-7.  A key or a value
+    that reads back as NaN reaches all that see it, and nothing else."""
     what = "attention_4bit"
     device = q.get_device()
     if device < 0 or out.get_device() != device or k_tiles.get_device() != device or v_tiles.get_device() != device or \
